@@ -68,7 +68,12 @@ enum wq_status {
     WQ_E_GROUP_MODE = 19,    /* "group_size must be None, 0, or positive" (quant.py:75-76) */
     WQ_E_LD = 20,            /* output row stride smaller than the row length */
     WQ_E_NOALLOC_LIMIT = 21, /* problem needs more scratch than wq_dequant_gemm_f32_noalloc holds */
-    WQ_E_OUTPUTS = 22        /* output count outside [1, WQ_MAX_OUTPUTS] */
+    WQ_E_OUTPUTS = 22,       /* output count outside [1, WQ_MAX_OUTPUTS] */
+    WQ_E_DTYPE = 23,         /* an element type that is not a wq_dtype */
+    WQ_E_BLOCK_ROWS = 24,    /* block_rows is neither 1 nor 128 */
+    WQ_E_ROW_STRIDE = 25,    /* a row stride smaller than the row length, or a negative scale stride */
+    WQ_E_CODES_ALIGN = 26,   /* product operand codes not 16-byte aligned, or rows not a multiple of 16 bytes apart */
+    WQ_E_INNER = 27          /* inner dimensions of a product differ */
 };
 
 /* Message for a status code (static storage; never NULL). */
@@ -336,6 +341,68 @@ WQ_API int wq_dequant_gemm_f32_multi(const float* x, int64_t B, int64_t K,
                                      const float* bias,
                                      void* workspace, size_t workspace_bytes,
                                      void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Blocks of 8-bit floating point (e4m3: 4 exponent and 3 mantissa bits,     */
+/* largest value 448, no infinity) and the linear layer made of them. No     */
+/* counterpart in ptqkit. An operand is                                      */
+/*   codes   uint8 [rows, cols], rows `ld` bytes apart                       */
+/*   scales  fp32, one per block: block_rows = 1: 128 values of a row;       */
+/*           block_rows = 128: a 128 x 128 tile. The scale of element (r, c) */
+/*           is scales[(r / block_rows) * s_row + (c / 128) * s_col]; any    */
+/*           non-negative strides. The last block of a row or column may be  */
+/*           short.                                                          */
+/* and stands for code * scale. The products take any finite fp32 scales     */
+/* whose product is finite too. Codes of a product's operand start on a      */
+/* 16-byte boundary and ld is a multiple of 16 (pad the rows; what the       */
+/* padding holds is not read as a value). Sums are held in fp32; every       */
+/* result is rounded once to its type and the same on every call.            */
+/* ------------------------------------------------------------------------ */
+enum wq_dtype { WQ_F32 = 0, WQ_F16 = 1, WQ_BF16 = 2 };
+
+/* Quantizes x [rows, cols] (row stride ldx elements). The scale of a block   */
+/* is the least power of two s >= 2^-117 with max|x| <= 448 s over the        */
+/* block's finite values, and 1 for a block of zeros; a code is the e4m3      */
+/* value nearest to x / s, ties to even. NaN and infinities become the NaN    */
+/* code 0x7f.                                                                */
+WQ_API int wq_fp8_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int block_rows,
+                           uint8_t* codes, int64_t ld, float* scales, int64_t s_row, int64_t s_col, void* stream);
+/* out [rows, cols] (row stride ldo elements) = code * scale. */
+WQ_API int wq_fp8_dequantize(const uint8_t* codes, int64_t rows, int64_t cols, int64_t ld, int block_rows,
+                             const float* scales, int64_t s_row, int64_t s_col, void* out, int out_type,
+                             int64_t ldo, void* stream);
+/* out [M, N] = a w^T (+ bias), the sum over each block of 128 scaled by the   */
+/* two blocks' scales: a [M, K] with block_rows 1, w [w_rows, w_cols] with     */
+/* block_rows 128. transpose = 0: w is [N, K] (a layer's forward product);     */
+/* transpose = 1: w is [K, N] (its input gradient, from the same stored        */
+/* weight). bias [N] of bias_type, or NULL. out has row stride ldo elements.   */
+WQ_API size_t wq_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+WQ_API int wq_fp8_gemm(const uint8_t* a, int64_t M, int64_t K, int64_t lda, const float* a_scales, int64_t as_row,
+                       int64_t as_col, const uint8_t* w, int64_t w_rows, int64_t w_cols, int64_t ldw,
+                       const float* w_scales, int64_t ws_row, int64_t ws_col, int transpose, const void* bias,
+                       int bias_type, void* out, int out_type, int64_t ldo, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* The same with a still in 16 or 32 bits: x [M, K] is quantized as            */
+/* wq_fp8_quantize does (block_rows 1) on its way into the product.            */
+WQ_API size_t wq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+WQ_API int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_t ldx, const uint8_t* w,
+                         int64_t w_rows, int64_t w_cols, int64_t ldw, const float* w_scales, int64_t ws_row,
+                         int64_t ws_col, int transpose, const void* bias, int bias_type, void* out, int out_type,
+                         int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
+/* dw [N, K] = sum_m dy[m, n] x^[m, k]: the weight gradient of a layer from the */
+/* 8-bit checkpoint of its input, x^ = code * scale with block_rows 1. dy       */
+/* [M, N] has row stride ldy. Scales that are powers of two (wq_fp8_quantize's) */
+/* make x^ exact in bf16, the product's operand type; with other scales x^ is   */
+/* rounded to bf16. accumulate != 0 adds to dw's values.                        */
+WQ_API size_t wq_fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type);
+WQ_API int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy, const uint8_t* codes,
+                              int64_t K, int64_t ld, const float* scales, int64_t s_row, int64_t s_col, void* dw,
+                              int dw_type, int64_t ldw, int accumulate, void* workspace, size_t workspace_bytes,
+                              void* stream);
+/* out [cols] = the sum of x [rows, cols] over its rows, in fp32, rounded once:  */
+/* the layer's bias gradient.                                                   */
+WQ_API int wq_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out,
+                         int out_type, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,16 @@ from .compressed import (
     save_compressed,
     state_dict_nbytes,
 )
-from .convert import iter_targets, quantize_model, weight_out_in
+from .convert import fp8_model, iter_targets, quantize_model, weight_out_in
+from .fp8 import (
+    Fp8Blocks,
+    Fp8Linear,
+    dequantize_fp8,
+    fp8_gemm,
+    fp8_linear,
+    fp8_weight_grad,
+    quantize_fp8,
+)
 from .gemm import dequant_gemm, kernel_info
 from .linear import QuantizedLinear
 from .pack import pack_int4, unpack_int4
@@ -41,6 +50,8 @@ from .quant import (
 __version__ = "0.1.0"
 
 __all__ = [
+    "Fp8Blocks",
+    "Fp8Linear",
     "Method",
     "QuantConfig",
     "QuantizedLinear",
@@ -49,8 +60,13 @@ __all__ = [
     "assemble_quantized",
     "compressed_state",
     "dequant_gemm",
+    "dequantize_fp8",
     "dequantize_weight",
     "element_scales",
+    "fp8_gemm",
+    "fp8_linear",
+    "fp8_model",
+    "fp8_weight_grad",
     "iter_targets",
     "kernel_info",
     "load_compressed",
@@ -58,6 +74,7 @@ __all__ = [
     "matrix_nbytes",
     "pack_int4",
     "payload_nbytes",
+    "quantize_fp8",
     "quantize_model",
     "quantize_weight",
     "read_compressed",

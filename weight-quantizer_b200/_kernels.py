@@ -24,7 +24,8 @@ LIB_PATH = os.path.join(_HERE, "libwq_b200.so")
 
 WQ_OK = 0
 WQ_E_CUDA = 14
-_ARG_ERRORS_AS_VALUEERROR = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 15, 16, 17, 18, 19, 20, 21, 22}
+_ARG_ERRORS_AS_VALUEERROR = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 15, 16, 17, 18, 19, 20, 21, 22, 23, 24, 25, 26,
+                             27}
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -83,6 +84,26 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
          _int, _int, _vp, _int, _i64, _vp, _vp, _vp, _sz, _vp],
     ),
+    "wq_fp8_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "wq_fp8_dequantize": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp, _int, _i64, _vp]),
+    "wq_fp8_gemm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "wq_fp8_gemm": (
+        _int,
+        [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _int, _vp, _int,
+         _vp, _int, _i64, _vp, _sz, _vp],
+    ),
+    "wq_fp8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "wq_fp8_linear": (
+        _int,
+        [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _int, _vp, _int,
+         _vp, _int, _i64, _vp, _sz, _vp],
+    ),
+    "wq_fp8_weight_grad_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "wq_fp8_weight_grad": (
+        _int,
+        [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _i64, _int, _vp, _sz, _vp],
+    ),
+    "wq_column_sum": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _vp]),
 }
 
 MAX_OUTPUTS = 8
@@ -656,3 +677,203 @@ def chol_inverse_upper(a: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check(library().wq_chol_inverse_upper_f64(_ptr(a), n, int(a.stride(0)), _ptr(u), n, _ptr(ws), ws_bytes,
                                                _ptr(info), _stream(dev)))
     return u, info
+
+
+# ---- blocks of 8-bit floating point -------------------------------------------
+
+FP8_BLOCK = 128
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # wq_dtype
+
+
+def _dtype(t: torch.dtype, what: str) -> int:
+    code = _DTYPES.get(t)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t}")
+    return code
+
+
+class _on:
+    """Makes a tensor's device the current one for a launch (nothing to do when it already is)."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device: torch.device) -> None:
+        self.index = device.index
+
+    def __enter__(self) -> None:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc: object) -> None:
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [rows, cols] with unit column stride and rows that do not overlap (a copy where x has neither)."""
+    if x.stride(1) == 1 and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1):
+        return x
+    return x if x.shape[1] == 1 and x.stride(0) >= 1 else x.contiguous()
+
+
+def _ld(x: torch.Tensor) -> int:
+    return int(x.stride(0)) if x.shape[0] > 1 else max(int(x.shape[1]), 1)
+
+
+def _codes_arg(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Codes as the products read them (16-byte aligned, rows a multiple of 16 bytes apart) and their row stride:
+    codes laid out otherwise are copied."""
+    rows, cols = codes.shape
+    if codes.numel() == 0:
+        return codes, (cols + 15) // 16 * 16
+    if codes.data_ptr() % 16 == 0 and (codes.stride(1) == 1 or cols == 1):
+        if rows == 1:
+            return codes, (cols + 15) // 16 * 16
+        if codes.stride(0) % 16 == 0 and codes.stride(0) >= cols:
+            return codes, int(codes.stride(0))
+    pitch = (cols + 15) // 16 * 16
+    kept = torch.empty((rows, pitch), dtype=torch.uint8, device=codes.device)
+    kept[:, :cols].copy_(codes.view(torch.uint8) if codes.stride(1) == 1 or cols == 1
+                         else codes.contiguous().view(torch.uint8))
+    return kept, pitch
+
+
+def _workspace(n: int, dev: torch.device) -> torch.Tensor | None:
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
+
+
+def _after_fp8(status: int) -> None:
+    if status != WQ_OK:
+        _check(status)
+    if _fault_check and not torch.cuda.is_current_stream_capturing():
+        _raise_on_fault()
+
+
+def fp8_quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of x [rows, cols]; codes are a view of rows padded to 16 bytes."""
+    x_type = _dtype(x.dtype, "x")
+    dev = _cuda_device([x])
+    x = _rows(x)
+    rows, cols = x.shape
+    pitch = (cols + 15) // 16 * 16
+    nb = (cols + FP8_BLOCK - 1) // FP8_BLOCK
+    codes = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=dev)
+    if block_rows == 1:
+        scales = torch.empty((nb, rows), dtype=torch.float32, device=dev).t()
+    else:
+        scales = torch.empty(((rows + FP8_BLOCK - 1) // FP8_BLOCK, nb), dtype=torch.float32, device=dev)
+    with _on(dev):
+        status = library().wq_fp8_quantize(
+            x.data_ptr(), x_type, rows, cols, _ld(x), block_rows, codes.data_ptr(), pitch, scales.data_ptr(),
+            scales.stride(0), scales.stride(1), _stream(dev))
+    _check(status)
+    return (codes if pitch == cols else codes[:, :cols]), scales
+
+
+def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, block_rows: int, dtype: torch.dtype) -> torch.Tensor:
+    """code * scale as a dense [rows, cols] tensor of ``dtype``."""
+    out_type = _dtype(dtype, "dtype")
+    dev = _cuda_device([codes, scales])
+    codes = _rows(codes)
+    rows, cols = codes.shape
+    out = torch.empty((rows, cols), dtype=dtype, device=dev)
+    with _on(dev):
+        _check(library().wq_fp8_dequantize(
+            codes.data_ptr(), rows, cols, _ld(codes), block_rows, scales.data_ptr(), scales.stride(0),
+            scales.stride(1), out.data_ptr(), out_type, max(cols, 1), _stream(dev)))
+    return out
+
+
+def _out_arg(out: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype,
+             dev: torch.device) -> tuple[torch.Tensor, int]:
+    if out is None:
+        return torch.empty((rows, cols), dtype=dtype, device=dev), max(cols, 1)
+    if out.dtype != dtype or out.device != dev or tuple(out.shape) != (rows, cols):
+        raise ValueError(f"out must be a {dtype} [{rows}, {cols}] tensor on the inputs' device")
+    if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+        raise ValueError("out must have unit column stride and rows that do not overlap")
+    return out, (int(out.stride(0)) if rows > 1 else max(cols, 1))
+
+
+def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor,
+             transpose: bool, bias: torch.Tensor | None, out_dtype: torch.dtype,
+             out: torch.Tensor | None) -> torch.Tensor:
+    """a w^T (+ bias), or a w with ``transpose``: a [M, K] codes with their scales, or (``a_scales`` None) a 16- or
+    32-bit matrix that the call quantizes."""
+    out_type = _dtype(out_dtype, "out_dtype")
+    dev = _cuda_device([a, w, w_scales] + ([] if a_scales is None else [a_scales]))
+    M, K = a.shape
+    w_rows, w_cols = w.shape
+    N = w_cols if transpose else w_rows
+    if (w_rows if transpose else w_cols) != K:
+        raise ValueError(f"a has trailing dim {K}, weight expects {w_rows if transpose else w_cols}")
+    bias_type = 0
+    if bias is not None:
+        bias_type = _dtype(bias.dtype, "bias")
+        if bias.device != dev:
+            raise ValueError("bias must be on the inputs' device")
+        bias = bias.reshape(-1).contiguous()
+        if bias.numel() != N:
+            raise ValueError("bias does not match the output's columns")
+    y, ldo = _out_arg(out, M, N, out_dtype, dev)
+    w, ldw = _codes_arg(w)
+    lib = library()
+    with _on(dev):
+        if a_scales is None:
+            x_type = _dtype(a.dtype, "a")
+            a = _rows(a)
+            nws = lib.wq_fp8_linear_workspace_bytes(M, N, K)
+            ws = _workspace(nws, dev)
+            status = lib.wq_fp8_linear(
+                a.data_ptr(), x_type, M, K, _ld(a), w.data_ptr(), w_rows, w_cols, ldw, w_scales.data_ptr(),
+                w_scales.stride(0), w_scales.stride(1), int(transpose), _ptr(bias), bias_type, y.data_ptr(), out_type,
+                ldo, _ptr(ws), nws, _stream(dev))
+        else:
+            a, lda = _codes_arg(a)
+            nws = lib.wq_fp8_gemm_workspace_bytes(M, N, K)
+            ws = _workspace(nws, dev)
+            status = lib.wq_fp8_gemm(
+                a.data_ptr(), M, K, lda, a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), w.data_ptr(),
+                w_rows, w_cols, ldw, w_scales.data_ptr(), w_scales.stride(0), w_scales.stride(1), int(transpose),
+                _ptr(bias), bias_type, y.data_ptr(), out_type, ldo, _ptr(ws), nws, _stream(dev))
+        _after_fp8(status)
+    return y
+
+
+def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype,
+                    out: torch.Tensor | None, accumulate: bool) -> torch.Tensor:
+    """dw [N, K] = dy^T (code * scale), added to ``out`` with ``accumulate``."""
+    dy_type = _dtype(dy.dtype, "dy")
+    out_type = _dtype(out_dtype, "out_dtype")
+    dev = _cuda_device([dy, codes, scales])
+    M, N = dy.shape
+    if codes.shape[0] != M:
+        raise ValueError(f"dy has {M} rows, the checkpoint {codes.shape[0]}")
+    K = codes.shape[1]
+    dw, ldw = _out_arg(out, N, K, out_dtype, dev)
+    dy = _rows(dy)
+    codes, ld = _codes_arg(codes)
+    lib = library()
+    nws = lib.wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type)
+    with _on(dev):
+        ws = _workspace(nws, dev)
+        status = lib.wq_fp8_weight_grad(
+            dy.data_ptr(), dy_type, M, N, _ld(dy), codes.data_ptr(), K, ld, scales.data_ptr(), scales.stride(0),
+            scales.stride(1), dw.data_ptr(), out_type, ldw, int(accumulate), _ptr(ws), nws, _stream(dev))
+        _after_fp8(status)
+    return dw
+
+
+def column_sum(x: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    """The sum of x [rows, cols] over its rows, in fp32, rounded once to ``out_dtype``."""
+    x_type = _dtype(x.dtype, "x")
+    out_type = _dtype(out_dtype, "out_dtype")
+    dev = _cuda_device([x])
+    x = _rows(x)
+    rows, cols = x.shape
+    out = torch.empty(cols, dtype=out_dtype, device=dev)
+    with _on(dev):
+        _check(library().wq_column_sum(x.data_ptr(), x_type, rows, cols, _ld(x), out.data_ptr(), out_type,
+                                       _stream(dev)))
+    return out

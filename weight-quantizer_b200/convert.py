@@ -34,6 +34,7 @@ from torch import nn
 
 from . import _kernels
 from .awq import awq_quantize, channel_mean_abs
+from .fp8 import Fp8Linear
 from .gptq import gptq_quantize
 from .linear import QuantizedLinear
 from .quant import Method, QuantConfig, QuantizedWeight, quantize_weight
@@ -261,3 +262,29 @@ def quantize_model(
             else:
                 layer.clear_cache()
     return done[0] if root_only else model
+
+
+def fp8_model(model: nn.Module, *, freeze: bool = False) -> nn.Module:
+    """Replace every nn.Linear and Conv1D of ``model`` in place by an ``Fp8Linear`` over
+    the same weight and bias: 8-bit operands in both directions, 8-bit checkpoints of
+    the layers' inputs. ``freeze`` keeps the weights as 8-bit tiles only, for serving.
+    A model that is itself the only target comes back as the replacement layer. An
+    nn.Linear's parameters stay the same objects (ties and optimizers keep them); a
+    Conv1D's weight is transposed into a new parameter. No ptqkit counterpart."""
+    if any(p.device.type != "cuda" for p in model.parameters()):
+        raise RuntimeError("fp8_model expects CUDA parameters")
+    root: nn.Module = model
+    for name, module in iter_targets(model):
+        if isinstance(module, nn.Linear):
+            layer = Fp8Linear.from_linear(module)
+        else:
+            bias = getattr(module, "bias", None)
+            layer = Fp8Linear(weight_out_in(module), bias if isinstance(bias, torch.Tensor) else None)
+        layer.train(module.training)
+        if freeze:
+            layer.freeze()
+        if name == "":
+            root = layer
+        else:
+            _set_module(model, name, layer)
+    return root

@@ -95,6 +95,10 @@ int cuda_fail(cudaError_t e) {
 }
 
 constexpr int64_t kMaxDim = ((int64_t)1 << 31) - 1;
+// 8-bit floating-point operands: rows and columns as far as the launch grids
+// and 32-bit tile coordinates reach.
+constexpr int64_t kMaxFp8Rows = (int64_t)1 << 22;
+constexpr int64_t kMaxFp8Cols = (int64_t)1 << 22;
 
 }  // namespace
 
@@ -126,6 +130,11 @@ const char* wq_status_string(int status) {
         case WQ_E_NOALLOC_LIMIT:
             return "problem needs more scratch than the no-allocation entry point holds; use wq_dequant_gemm_f32";
         case WQ_E_OUTPUTS: return "output count must be between 1 and WQ_MAX_OUTPUTS";
+        case WQ_E_DTYPE: return "element type must be fp32, fp16 or bf16";
+        case WQ_E_BLOCK_ROWS: return "block_rows must be 1 or 128";
+        case WQ_E_ROW_STRIDE: return "row stride is smaller than the row length, or a scale stride is negative";
+        case WQ_E_CODES_ALIGN: return "codes must be 16-byte aligned with rows a multiple of 16 bytes apart";
+        case WQ_E_INNER: return "inner dimensions do not match";
         default: return "unknown status";
     }
 }
@@ -561,6 +570,161 @@ int wq_chol_inverse_upper_f64(const double* a, int64_t n, int64_t lda, double* u
     if (n > 46340) return WQ_E_TOO_LARGE;   // n * n elements indexed by the rotation's grid
     cudaError_t e = wq::launch_chol_inverse_upper(a, n, lda, u, ldu, static_cast<double*>(workspace), info,
                                                   static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+static bool fp8_type_ok(int t) { return t == WQ_F32 || t == WQ_F16 || t == WQ_BF16; }
+
+int wq_fp8_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int block_rows,
+                    uint8_t* codes, int64_t ld, float* scales, int64_t s_row, int64_t s_col, void* stream) {
+    if (!fp8_type_ok(x_type)) return WQ_E_DTYPE;
+    if (block_rows != 1 && block_rows != wq::kFp8Block) return WQ_E_BLOCK_ROWS;
+    if (rows < 0 || cols < 0) return WQ_E_NEG_DIM;
+    if (ldx < cols || ld < cols || s_row < 0 || s_col < 0) return WQ_E_ROW_STRIDE;
+    if (rows > kMaxDim || cols > kMaxFp8Cols) return WQ_E_TOO_LARGE;
+    if (block_rows != 1 && ((rows + 127) / 128) * ((cols + 127) / 128) > kMaxDim) return WQ_E_TOO_LARGE;
+    if (rows == 0 || cols == 0) return WQ_OK;
+    if (x == nullptr || codes == nullptr || scales == nullptr) return WQ_E_NULL;
+    const wq::Fp8Quantize q{x, x_type, rows, cols, ldx, codes, ld, scales, s_row, s_col, block_rows};
+    cudaError_t e = wq::launch_fp8_quantize(q, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+int wq_fp8_dequantize(const uint8_t* codes, int64_t rows, int64_t cols, int64_t ld, int block_rows,
+                      const float* scales, int64_t s_row, int64_t s_col, void* out, int out_type, int64_t ldo,
+                      void* stream) {
+    if (!fp8_type_ok(out_type)) return WQ_E_DTYPE;
+    if (block_rows != 1 && block_rows != wq::kFp8Block) return WQ_E_BLOCK_ROWS;
+    if (rows < 0 || cols < 0) return WQ_E_NEG_DIM;
+    if (ld < cols || ldo < cols || s_row < 0 || s_col < 0) return WQ_E_ROW_STRIDE;
+    if (rows > kMaxDim || cols > kMaxFp8Cols) return WQ_E_TOO_LARGE;
+    if (rows == 0 || cols == 0) return WQ_OK;
+    if (codes == nullptr || scales == nullptr || out == nullptr) return WQ_E_NULL;
+    const wq::Fp8Operand a{codes, rows, cols, ld, scales, s_row, s_col, block_rows};
+    cudaError_t e = wq::launch_fp8_values(a, out, out_type, ldo, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+// What wq_fp8_gemm and wq_fp8_linear check alike: the weight, the bias, the
+// output and the inner dimension.
+static int fp8_check_product(int64_t M, int64_t K, const uint8_t* w, int64_t w_rows, int64_t w_cols, int64_t ldw,
+                             int64_t ws_row, int64_t ws_col, int transpose, const void* bias, int bias_type,
+                             int out_type, int64_t ldo) {
+    if (!fp8_type_ok(out_type) || (bias != nullptr && !fp8_type_ok(bias_type))) return WQ_E_DTYPE;
+    if (M < 0 || K < 0 || w_rows < 0 || w_cols < 0) return WQ_E_NEG_DIM;
+    const int64_t N = transpose ? w_cols : w_rows;
+    if ((transpose ? w_rows : w_cols) != K) return WQ_E_INNER;
+    if (ldw < w_cols || ws_row < 0 || ws_col < 0) return WQ_E_ROW_STRIDE;
+    if (ldo < N) return WQ_E_LD;
+    if (ldw % 16 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0) return WQ_E_CODES_ALIGN;
+    if (M > kMaxFp8Rows || K > kMaxFp8Cols || N > kMaxFp8Cols) return WQ_E_TOO_LARGE;
+    return WQ_OK;
+}
+
+size_t wq_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : wq::fp8_gemm_workspace_bytes(M, N, K);
+}
+
+int wq_fp8_gemm(const uint8_t* a, int64_t M, int64_t K, int64_t lda, const float* a_scales, int64_t as_row,
+                int64_t as_col, const uint8_t* w, int64_t w_rows, int64_t w_cols, int64_t ldw, const float* w_scales,
+                int64_t ws_row, int64_t ws_col, int transpose, const void* bias, int bias_type, void* out,
+                int out_type, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    const int bad = fp8_check_product(M, K, w, w_rows, w_cols, ldw, ws_row, ws_col, transpose, bias, bias_type,
+                                      out_type, ldo);
+    if (bad != WQ_OK) return bad;
+    if (lda < K || as_row < 0 || as_col < 0) return WQ_E_ROW_STRIDE;
+    if (lda % 16 != 0 || (reinterpret_cast<uintptr_t>(a) & 15) != 0) return WQ_E_CODES_ALIGN;
+    const int64_t N = transpose ? w_cols : w_rows;
+    if (M == 0 || N == 0) return WQ_OK;
+    if (out == nullptr) return WQ_E_NULL;
+    if (K > 0 && (a == nullptr || a_scales == nullptr || w == nullptr || w_scales == nullptr)) return WQ_E_NULL;
+    const size_t need = wq_fp8_gemm_workspace_bytes(M, N, K);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
+    const wq::Fp8Operand ao{a, M, K, lda, a_scales, as_row, as_col, 1};
+    const wq::Fp8Operand wo{w, w_rows, w_cols, ldw, w_scales, ws_row, ws_col, wq::kFp8Block};
+    const wq::Fp8Gemm g{ao, wo, transpose ? 1 : 0, M, N, K, bias, bias_type, out, out_type, ldo};
+    cudaError_t e = wq::launch_fp8_gemm(g, workspace, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+// Workspace of wq_fp8_linear: the codes of x (rows padded to 16 bytes), its
+// scales (one block's values of all rows side by side), the product's own.
+static size_t fp8_codes_bytes(int64_t M, int64_t K) { return ((size_t)M * ((K + 15) / 16 * 16) + 255) / 256 * 256; }
+static size_t fp8_scales_bytes(int64_t M, int64_t K) {
+    return ((size_t)M * ((K + 127) / 128) * sizeof(float) + 255) / 256 * 256;
+}
+
+size_t wq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return fp8_codes_bytes(M, K) + fp8_scales_bytes(M, K) + wq::fp8_gemm_workspace_bytes(M, N, K);
+}
+
+int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, int64_t w_rows,
+                  int64_t w_cols, int64_t ldw, const float* w_scales, int64_t ws_row, int64_t ws_col, int transpose,
+                  const void* bias, int bias_type, void* out, int out_type, int64_t ldo, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    if (!fp8_type_ok(x_type)) return WQ_E_DTYPE;
+    const int bad = fp8_check_product(M, K, w, w_rows, w_cols, ldw, ws_row, ws_col, transpose, bias, bias_type,
+                                      out_type, ldo);
+    if (bad != WQ_OK) return bad;
+    if (ldx < K) return WQ_E_ROW_STRIDE;
+    const int64_t N = transpose ? w_cols : w_rows;
+    if (M == 0 || N == 0) return WQ_OK;
+    if (out == nullptr) return WQ_E_NULL;
+    if (K > 0 && (x == nullptr || w == nullptr || w_scales == nullptr)) return WQ_E_NULL;
+    const size_t need = wq_fp8_linear_workspace_bytes(M, N, K);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return WQ_E_WORKSPACE;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    float* scales = reinterpret_cast<float*>(codes + fp8_codes_bytes(M, K));
+    void* rest = codes + fp8_codes_bytes(M, K) + fp8_scales_bytes(M, K);
+    const int64_t ld = (K + 15) / 16 * 16;
+    const wq::Fp8Operand ao{codes, M, K, ld, scales, 1, M, 1};
+    const wq::Fp8Operand wo{w, w_rows, w_cols, ldw, w_scales, ws_row, ws_col, wq::kFp8Block};
+    const wq::Fp8Gemm g{ao, wo, transpose ? 1 : 0, M, N, K, bias, bias_type, out, out_type, ldo};
+    if (K > 0) {
+        const wq::Fp8Quantize q{x, x_type, M, K, ldx, codes, ld, scales, 1, M, 1};
+        cudaError_t e = wq::launch_fp8_quantize(q, s);
+        if (e != cudaSuccess) return cuda_fail(e);
+    }
+    cudaError_t e = wq::launch_fp8_gemm(g, rest, s);
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+size_t wq_fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type) {
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : wq::fp8_weight_grad_workspace_bytes(M, N, K, dy_type);
+}
+
+int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy, const uint8_t* codes, int64_t K,
+                       int64_t ld, const float* scales, int64_t s_row, int64_t s_col, void* dw, int dw_type,
+                       int64_t ldw, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!fp8_type_ok(dy_type) || !fp8_type_ok(dw_type)) return WQ_E_DTYPE;
+    if (M < 0 || N < 0 || K < 0) return WQ_E_NEG_DIM;
+    if (ldy < N || ld < K || s_row < 0 || s_col < 0) return WQ_E_ROW_STRIDE;
+    if (ldw < K) return WQ_E_LD;
+    if (ld % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15) != 0) return WQ_E_CODES_ALIGN;
+    if (M > kMaxFp8Rows || N > kMaxFp8Cols || K > kMaxFp8Cols) return WQ_E_TOO_LARGE;
+    if (N == 0 || K == 0) return WQ_OK;
+    if (dw == nullptr) return WQ_E_NULL;
+    if (M > 0 && (dy == nullptr || codes == nullptr || scales == nullptr)) return WQ_E_NULL;
+    const size_t need = wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
+    const wq::Fp8Operand ao{codes, M, K, ld, scales, s_row, s_col, 1};
+    const wq::Fp8WeightGrad g{dy, dy_type, ldy, ao, M, N, K, dw, dw_type, ldw, accumulate ? 1 : 0};
+    cudaError_t e = wq::launch_fp8_weight_grad(g, workspace, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WQ_OK : cuda_fail(e);
+}
+
+int wq_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out, int out_type,
+                  void* stream) {
+    if (!fp8_type_ok(x_type) || !fp8_type_ok(out_type)) return WQ_E_DTYPE;
+    if (rows < 0 || cols < 0) return WQ_E_NEG_DIM;
+    if (ldx < cols) return WQ_E_ROW_STRIDE;
+    if (rows > kMaxDim || cols > kMaxDim) return WQ_E_TOO_LARGE;
+    if (cols == 0) return WQ_OK;
+    if (out == nullptr || (rows > 0 && x == nullptr)) return WQ_E_NULL;
+    cudaError_t e = wq::launch_column_sum(x, x_type, rows, cols, ldx, out, out_type, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
 

@@ -1,0 +1,257 @@
+// Blocks of 8-bit floating point: quantize, the reverse, and the column sums
+// of a layer's upstream gradient (its bias gradient).
+//
+//   block b of x (128 values of a row, or a 128 x 128 tile):
+//     s_b = 2^k, the least k >= -117 with max|x| <= 448 * 2^k   (1 if the block is 0)
+//     c   = e4m3(x / s_b), nearest, ties to even; x / s_b is exact (a shift of
+//           the exponent), so each code is the e4m3 value nearest to x / s_b
+//
+// Why a power of two: the codes are floating point, so a scale up to twice as
+// large costs no relative precision above the least codes, while the division
+// and the product code * scale become exact: the weight gradient reads
+// code * scale as a bf16 operand without a rounding.
+//
+// Bound: HBM. Bytes per value: the input's 2 or 4, 1 for the code, 4/128 (rows)
+// or 4/16384 (tiles) for the scale.
+#include "fp8_types.cuh"
+#include "kernels.h"
+
+namespace wq {
+namespace {
+
+// Eight consecutive values of a row as fp32; `n` of them exist (the others
+// read as 0). VEC: the eight are 16-byte aligned in memory.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+    if (VEC && n >= 8) {
+        constexpr int W = (int)(8 * sizeof(T) / 16);
+        uint4 r[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) r[i] = ld_stream_v4(reinterpret_cast<const uint4*>(p) + i);
+        const T* e = reinterpret_cast<const T*>(r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(p[i]) : 0.0f;
+    }
+}
+
+// Codes of eight values; `n` of them are written. VEC: 8-byte aligned.
+__device__ __forceinline__ void store8(uint8_t* p, int n, const float (&v)[8], float inv, bool vec) {
+    uint2 w;
+    w.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+    w.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+    if (vec && n >= 8) {
+        *reinterpret_cast<uint2*>(p) = w;
+    } else {
+        const uint64_t u = (uint64_t)w.x | ((uint64_t)w.y << 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = (uint8_t)(u >> (8 * i));
+    }
+}
+
+constexpr int kRowsPerCta = 16;     // one half-warp per row
+constexpr int kBlocksPerThread = 4; // consecutive blocks of the row in flight
+
+// One scale per 128 values of a row: 16 lanes hold a block (8 values each). A
+// CTA takes 16 rows, so that the scales of one block column, which lie side by
+// side for consecutive rows, are written as 64 contiguous bytes.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                       int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc,
+                                                       bool vec_out, float* __restrict__ scales, int64_t s_row,
+                                                       int64_t s_col) {
+    const int64_t row = (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 4);
+    const int sub = threadIdx.x & 15;
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block;
+    const int64_t j0 = (int64_t)blockIdx.y * kBlocksPerThread;
+    const bool live = row < rows;
+    float v[kBlocksPerThread][8];
+#pragma unroll
+    for (int i = 0; i < kBlocksPerThread; ++i) {
+        const int64_t c = (j0 + i) * kFp8Block + sub * 8;
+        const int64_t left = live ? cols - c : 0;
+        load8<T, VEC>(x + row * ldx + c, left >= 8 ? 8 : (left > 0 ? (int)left : 0), v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kBlocksPerThread; ++i) {
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e = fp8_scale_exponent(m);
+        const int64_t j = j0 + i;
+        const int64_t c = j * kFp8Block + sub * 8;
+        const int64_t left = live ? cols - c : 0;
+        if (left > 0) store8(codes + row * ldc + c, left >= 8 ? 8 : (int)left, v[i], pow2i(-e), vec_out);
+        if (live && j < nb && sub == 0) scales[row * s_row + j * s_col] = pow2i(e);
+    }
+}
+
+// One scale per 128 x 128 tile: a CTA holds the tile in registers (half-warp
+// h has rows h, h + 16, ...), so the input is read once.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_tiles_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                        int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc,
+                                                        bool vec_out, float* __restrict__ scales, int64_t s_row,
+                                                        int64_t s_col, int64_t nb) {
+    __shared__ float red[8];
+    const int64_t bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;
+    const int sub = threadIdx.x & 15;
+    const int64_t r0 = bi * kFp8Block + (threadIdx.x >> 4);
+    const int64_t c = bj * kFp8Block + sub * 8;
+    const int64_t left = cols - c;
+    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    float v[8][8];
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + 16 * i;
+        load8<T, VEC>(x + r * ldx + c, r < rows ? n : 0, v[i]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+    const int e = fp8_scale_exponent(m);
+    const float inv = pow2i(-e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + 16 * i;
+        if (r < rows && n > 0) store8(codes + r * ldc + c, n, v[i], inv, vec_out);
+    }
+    if (threadIdx.x == 0) scales[bi * s_row + bj * s_col] = pow2i(e);
+}
+
+// out = code * scale, rounded once to the output type.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_values_kernel(const uint8_t* __restrict__ codes, int64_t rows,
+                                                         int64_t cols, int64_t ldc, int block_rows,
+                                                         const float* __restrict__ scales, int64_t s_row,
+                                                         int64_t s_col, T* __restrict__ out, int64_t ldo,
+                                                         int64_t quads) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * quads;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / quads, c = (i - r * quads) * 4;
+        const float s = __ldg(scales + (r / block_rows) * s_row + (c / kFp8Block) * s_col);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (c + k < cols) out[r * ldo + c + k] = from_f32<T>(e4m3x2_values(codes[r * ldc + c + k]).x * s);
+    }
+}
+
+// out[n] = sum_m x[m, n] in fp32: a CTA takes 64 columns, 8 threads side by
+// side (8 columns each) times 32 row lanes; each thread adds its rows in
+// order, then the lanes are added in order (the same bits on every call).
+template <typename T, typename O, bool VEC>
+__global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                         int64_t ldx, O* __restrict__ out) {
+    __shared__ float part[32][65];
+    const int sub = threadIdx.x & 7, lane = threadIdx.x >> 3;
+    const int64_t c = (int64_t)blockIdx.x * 64 + sub * 8;
+    const int64_t left = cols - c;
+    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    float acc[8] = {};
+#pragma unroll 4
+    for (int64_t r = lane; r < rows; r += 32) {
+        float v[8];
+        load8<T, VEC>(x + r * ldx + c, n, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[lane][sub * 8 + k] = acc[k];
+    __syncthreads();
+    if (threadIdx.x < 64 && (int64_t)blockIdx.x * 64 + threadIdx.x < cols) {
+        float s = 0.0f;
+#pragma unroll
+        for (int l = 0; l < 32; ++l) s += part[l][threadIdx.x];
+        out[(int64_t)blockIdx.x * 64 + threadIdx.x] = from_f32<O>(s);
+    }
+}
+
+template <typename T>
+cudaError_t quantize_t(const Fp8Quantize& q, cudaStream_t s) {
+    const T* x = static_cast<const T*>(q.x);
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (q.ldx * (int64_t)sizeof(T)) % 16 == 0;
+    const bool vec_out = (reinterpret_cast<uintptr_t>(q.codes) & 7) == 0 && q.ldc % 8 == 0;
+    const int64_t nb = (q.cols + kFp8Block - 1) / kFp8Block;
+    if (q.block_rows == 1) {
+        const dim3 grid((unsigned)((q.rows + kRowsPerCta - 1) / kRowsPerCta),
+                        (unsigned)((nb + kBlocksPerThread - 1) / kBlocksPerThread));
+        if (vec)
+            fp8_rows_kernel<T, true><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out, q.scales,
+                                                          q.s_row, q.s_col);
+        else
+            fp8_rows_kernel<T, false><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out, q.scales,
+                                                           q.s_row, q.s_col);
+    } else {
+        const unsigned grid = (unsigned)((q.rows + kFp8Block - 1) / kFp8Block * nb);
+        if (vec)
+            fp8_tiles_kernel<T, true><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out,
+                                                           q.scales, q.s_row, q.s_col, nb);
+        else
+            fp8_tiles_kernel<T, false><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out,
+                                                            q.scales, q.s_row, q.s_col, nb);
+    }
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t values_t(const Fp8Operand& a, T* out, int64_t ldo, cudaStream_t s) {
+    const int64_t quads = (a.cols + 3) / 4;
+    const int64_t want = (a.rows * quads + 255) / 256;
+    const int64_t most = (int64_t)sm_count() * 32;
+    fp8_values_kernel<T><<<(unsigned)(want < most ? want : most), 256, 0, s>>>(
+        a.codes, a.rows, a.cols, a.ld, a.block_rows, a.scales, a.s_row, a.s_col, out, ldo, quads);
+    return cudaGetLastError();
+}
+
+template <typename T, typename O>
+cudaError_t column_sum_t(const T* x, int64_t rows, int64_t cols, int64_t ldx, O* out, cudaStream_t s) {
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
+    const unsigned grid = (unsigned)((cols + 63) / 64);
+    if (vec)
+        column_sum_kernel<T, O, true><<<grid, 256, 0, s>>>(x, rows, cols, ldx, out);
+    else
+        column_sum_kernel<T, O, false><<<grid, 256, 0, s>>>(x, rows, cols, ldx, out);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t column_sum_o(const T* x, int64_t rows, int64_t cols, int64_t ldx, void* out, int out_type,
+                         cudaStream_t s) {
+    if (out_type == kF16) return column_sum_t(x, rows, cols, ldx, static_cast<__half*>(out), s);
+    if (out_type == kBf16) return column_sum_t(x, rows, cols, ldx, static_cast<__nv_bfloat16*>(out), s);
+    return column_sum_t(x, rows, cols, ldx, static_cast<float*>(out), s);
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_quantize(const Fp8Quantize& q, cudaStream_t s) {
+    if (q.x_type == kF16) return quantize_t<__half>(q, s);
+    if (q.x_type == kBf16) return quantize_t<__nv_bfloat16>(q, s);
+    return quantize_t<float>(q, s);
+}
+
+cudaError_t launch_fp8_values(const Fp8Operand& a, void* out, int out_type, int64_t ldo, cudaStream_t s) {
+    if (out_type == kF16) return values_t(a, static_cast<__half*>(out), ldo, s);
+    if (out_type == kBf16) return values_t(a, static_cast<__nv_bfloat16*>(out), ldo, s);
+    return values_t(a, static_cast<float*>(out), ldo, s);
+}
+
+cudaError_t launch_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out,
+                              int out_type, cudaStream_t s) {
+    if (x_type == kF16) return column_sum_o(static_cast<const __half*>(x), rows, cols, ldx, out, out_type, s);
+    if (x_type == kBf16) return column_sum_o(static_cast<const __nv_bfloat16*>(x), rows, cols, ldx, out, out_type, s);
+    return column_sum_o(static_cast<const float*>(x), rows, cols, ldx, out, out_type, s);
+}
+
+}  // namespace wq

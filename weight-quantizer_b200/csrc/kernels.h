@@ -130,6 +130,66 @@ cudaError_t launch_chol_inverse_upper(const double* a, int64_t n, int64_t lda, d
 cudaError_t launch_gptq_tail(double* work, int64_t rows, int64_t ld, int64_t c0, int64_t ncols, const double* err,
                              int count, const double* hinv, int64_t ldh, int64_t s0, cudaStream_t s);
 
+// --- Blocks of 8-bit floating point (fp8_quant.cu, fp8_gemm.cu, fp8_wgrad.cu) ----
+constexpr int kF32 = 0, kF16 = 1, kBf16 = 2;   // wq_dtype
+constexpr int kFp8Block = 128;                 // values of a row under one scale, rows of a tile
+
+// e4m3 codes [rows, cols] (rows `ld` bytes apart) and the scale of each block
+// of block_rows x 128: scales[(r / block_rows) * s_row + (c / 128) * s_col].
+struct Fp8Operand {
+    const uint8_t* codes;
+    int64_t rows, cols, ld;
+    const float* scales;
+    int64_t s_row, s_col;
+    int block_rows;   // 1 or 128
+};
+struct Fp8Quantize {
+    const void* x;
+    int x_type;
+    int64_t rows, cols, ldx;
+    uint8_t* codes;
+    int64_t ldc;
+    float* scales;
+    int64_t s_row, s_col;
+    int block_rows;
+};
+cudaError_t launch_fp8_quantize(const Fp8Quantize& q, cudaStream_t s);
+cudaError_t launch_fp8_values(const Fp8Operand& a, void* out, int out_type, int64_t ldo, cudaStream_t s);
+cudaError_t launch_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out,
+                              int out_type, cudaStream_t s);
+
+// y[m, n] = sum_b sa[m, b] sum_{c in block b} a[m, c] w^(n, c) (+ bias[n]): a has
+// one scale per row and block, w one per 128 x 128 tile. w^ is w [N, K], or with
+// `transpose` its transpose (w [K, N]).
+struct Fp8Gemm {
+    Fp8Operand a, w;
+    int transpose;
+    int64_t M, N, K;
+    const void* bias;   // [N] or nullptr
+    int bias_type;
+    void* out;
+    int out_type;
+    int64_t ldo;
+};
+size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, cudaStream_t s);
+
+// dw[n, k] (+)= sum_m dy[m, n] x^[m, k], x^ the values of a with one scale per
+// row and block.
+struct Fp8WeightGrad {
+    const void* dy;   // [M, N]
+    int dy_type;
+    int64_t ldy;
+    Fp8Operand a;     // [M, K]
+    int64_t M, N, K;
+    void* out;        // [N, K]
+    int out_type;
+    int64_t ldo;
+    int accumulate;   // add to out's values
+};
+size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type);
+cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cudaStream_t s);
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
