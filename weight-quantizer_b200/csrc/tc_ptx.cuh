@@ -178,8 +178,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Relaxed: what it orders is tensor memory (tcgen05 fences on both sides); a
+// release would add a fence of all memory, which stalled each block's hand-off.
 __device__ __forceinline__ void arrive_in_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
     uint32_t ok;
