@@ -42,8 +42,9 @@ static_assert(kPairCtlRegs + 2 * kPairSumRegs <= 3 * kPairLaunchRegs, "register 
 
 struct PairSmem {
     static constexpr int BAR = kPairStages * kPairStage;
-    // full, empty per stage; sums full[2], empty[2]
-    static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 4);
+    // full and done per stage (done: the block's MMAs are over, so its operands
+    // may be replaced and its sums read); sums empty[2]
+    static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 2);
     static constexpr int TOTAL = TMEM_SLOT + 16;
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
 };
@@ -116,23 +117,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_addr(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int rank = (int)cluster_rank();
     auto bar = [&](int i) -> uint32_t { return sbase + L::BAR + 8u * (uint32_t)i; };
     auto full = [&](int s) { return bar(s); };
-    auto empty = [&](int s) { return bar(kPairStages + s); };
-    auto sums_full = [&](int b) { return bar(2 * kPairStages + b); };
-    auto sums_empty = [&](int b) { return bar(2 * kPairStages + 2 + b); };
+    auto done = [&](int s) { return bar(kPairStages + s); };
+    auto sums_empty = [&](int b) { return bar(2 * kPairStages + b); };
     launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
             mbar_init(full(s), 1);     // the even CTA's: its own arrival plus both CTAs' bytes
-            mbar_init(empty(s), 1);
+            mbar_init(done(s), 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(sums_full(b), 1);
+        for (int b = 0; b < 2; ++b)
             mbar_init(sums_empty(b), 16);   // the even CTA's: one arrival per summing warp of the pair
-        }
         fence_mbarrier_init();
     }
     if (warp == 1) tmem_alloc<2>(sbase + L::TMEM_SLOT, 512);
@@ -164,7 +162,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 tile_of(t, p, mt, nt);
                 const int m0 = mt * kPairTile + rank * 128, n0 = nt * kPairTile + rank * 128;
                 for (int b = 0; b < p.blocks; ++b) {
-                    if (!faulted && !mbar_wait_bounded(empty(s), ph)) give_up();
+                    if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
                     const uint32_t f = in_cta(full(s), 0);
                     if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
                     const uint32_t dst = sbase + (uint32_t)(s * kPairStage);
@@ -180,30 +178,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             // every copy this thread started has been read before the CTA goes
             // (a stage that was never filled passes at once)
             for (int i = 0; i < kPairStages; ++i) {
-                if (!mbar_wait_bounded(empty(s), ph)) atomicOr(p.fault, 1u);
+                if (!mbar_wait_bounded(done(s), ph)) atomicOr(p.fault, 1u);
                 if (++s == kPairStages) {
                     s = 0;
                     ph ^= 1u;
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp == 1 && rank == 0) {
             constexpr uint32_t idesc = mma_idesc(0, false, WT, 256, 256);
             const uint64_t desc0 = sw128_matrix(sbase);
             int s = 0;
             uint32_t ph = 0;
             for (int64_t i = 0; i < steps; ++i) {
                 const int buf = (int)(i & 1);
-                if (i >= 2 && !faulted && !wait_cluster_bounded(sums_empty(buf), (uint32_t)(((i >> 1) - 1) & 1)))
+                if (i >= 2 && !faulted && !mbar_wait_bounded(sums_empty(buf), (uint32_t)(((i >> 1) - 1) & 1)))
                     give_up();
-                if (!faulted && !wait_cluster_bounded(full(s), ph)) give_up();
+                if (!faulted && !mbar_wait_bounded(full(s), ph)) give_up();
+                __syncwarp();
                 tc_after();
-                const uint64_t da = desc0 + (uint64_t)(s * (kPairStage >> 4));
-                const uint64_t dw = da + (uint64_t)(kOperandBytes >> 4);
+                if (elect_one()) {
+                    const uint64_t da = desc0 + (uint64_t)(s * (kPairStage >> 4));
+                    const uint64_t dw = da + (uint64_t)(kOperandBytes >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)   // 32 codes: 32 bytes of a row, or 32 rows of 128 bytes
-                    mma_f8<2>(tmem + (uint32_t)(buf * 256), da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
-                mma_done<2>(empty(s));
-                mma_done<2>(sums_full(buf));
+                    for (int k = 0; k < 4; ++k)   // 32 codes: 32 bytes of a row, or 32 rows of 128 bytes
+                        mma_f8<2>(tmem + (uint32_t)(buf * 256), da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
+                    mma_done<2>(done(s));
+                }
+                __syncwarp();
                 if (++s == kPairStages) {
                     s = 0;
                     ph ^= 1u;
@@ -216,6 +217,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
         const uint32_t free0 = in_cta(sums_empty(0), 0);
         int64_t i = 0;
+        int s = 0;
+        uint32_t ph = 0;
         for (int t = first; t < tiles; t += pairs) {
             int mt, nt;
             tile_of(t, p, mt, nt);
@@ -236,29 +239,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 a1 = a2, w1 = w2, a2 = a3, w2 = w3;
                 if (b + 3 < p.blocks) a3 = __ldg(sa + (b + 3) * p.sa_col), w3 = __ldg(sw + (b + 3) * p.sw_k);
                 const uint64_t sc2 = pack2(sc, sc);
-                if (!faulted && !mbar_wait_bounded(sums_full(buf), (uint32_t)((i >> 1) & 1))) give_up();
+                if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
+                if (++s == kPairStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
                 __syncwarp();
                 tc_after();
-                uint32_t r0[32], r1[32];
-                tmem_ld(taddr + (uint32_t)(buf * 256), r0);
-                tmem_wait(r0);
-                tmem_ld(taddr + (uint32_t)(buf * 256 + 32), r1);
+                const uint32_t from = taddr + (uint32_t)(buf * 256);
+                uint64_t v[32];
+                tmem_pairs(from, v);
 #pragma unroll
-                for (int c = 0; c < 16; ++c) fma2(acc[c], pack2(r0[2 * c], r0[2 * c + 1]), sc2);
-                tmem_wait(r1);
-                tmem_ld(taddr + (uint32_t)(buf * 256 + 64), r0);
-#pragma unroll
-                for (int c = 0; c < 16; ++c) fma2(acc[16 + c], pack2(r1[2 * c], r1[2 * c + 1]), sc2);
-                tmem_wait(r0);
-                tmem_ld(taddr + (uint32_t)(buf * 256 + 96), r1);
-#pragma unroll
-                for (int c = 0; c < 16; ++c) fma2(acc[32 + c], pack2(r0[2 * c], r0[2 * c + 1]), sc2);
-                tmem_wait(r1);
+                for (int c = 0; c < 32; ++c) fma2(acc[c], v[c], sc2);
+                tmem_pairs(from + 64u, v);
                 tc_before();
                 __syncwarp();
                 if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
 #pragma unroll
-                for (int c = 0; c < 16; ++c) fma2(acc[48 + c], pack2(r1[2 * c], r1[2 * c + 1]), sc2);
+                for (int c = 0; c < 32; ++c) fma2(acc[32 + c], v[c], sc2);
             }
             if (m < p.M) {
 #pragma unroll
