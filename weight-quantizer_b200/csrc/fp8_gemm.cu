@@ -33,7 +33,7 @@ namespace {
 // the MMA's MN-major form of the same operand.
 
 constexpr int kPairTile = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 6;                      // even: each issuing warp has its own
 constexpr int kOperandBytes = 128 * 128;            // one operand of one CTA for one block
 constexpr int kPairStage = 2 * kOperandBytes;
 constexpr int kPairThreads = 384;
@@ -184,29 +184,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     ph ^= 1u;
                 }
             }
-        } else if (warp == 1 && rank == 0) {
+        } else if ((warp == 1 || warp == 2) && rank == 0) {
+            // even blocks by warp 1, odd ones by warp 2: a wait on a barrier takes
+            // about 170 cycles beside the MMAs' own reads of shared memory, and one
+            // warp's waits and its issue together take as long as a block's MMAs
             constexpr uint32_t idesc = mma_idesc(0, false, WT, 256, 256);
             const uint64_t desc0 = sw128_matrix(sbase);
-            int s = 0;
+            const int buf = warp - 1;
+            const uint32_t d = tmem + (uint32_t)(buf * 256);
+            int s = buf;
             uint32_t ph = 0;
-            for (int64_t i = 0; i < steps; ++i) {
-                const int buf = (int)(i & 1);
+            for (int64_t i = buf; i < steps; i += 2) {
+                if (!faulted && !mbar_wait_bounded(full(s), ph)) give_up();
+                const uint64_t da = desc0 + (uint64_t)(s * (kPairStage >> 4));
+                const uint64_t dw = da + (uint64_t)(kOperandBytes >> 4);
                 if (i >= 2 && !faulted && !mbar_wait_bounded(sums_empty(buf), (uint32_t)(((i >> 1) - 1) & 1)))
                     give_up();
-                if (!faulted && !mbar_wait_bounded(full(s), ph)) give_up();
                 __syncwarp();
                 tc_after();
                 if (elect_one()) {
-                    const uint64_t da = desc0 + (uint64_t)(s * (kPairStage >> 4));
-                    const uint64_t dw = da + (uint64_t)(kOperandBytes >> 4);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)   // 32 codes: 32 bytes of a row, or 32 rows of 128 bytes
-                        mma_f8<2>(tmem + (uint32_t)(buf * 256), da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
+                        mma_f8<2>(d, da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
                     mma_done<2>(done(s));
                 }
                 __syncwarp();
-                if (++s == kPairStages) {
-                    s = 0;
+                s += 2;
+                if (s >= kPairStages) {
+                    s = buf;
                     ph ^= 1u;
                 }
             }
@@ -239,15 +244,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 a1 = a2, w1 = w2, a2 = a3, w2 = w3;
                 if (b + 3 < p.blocks) a3 = __ldg(sa + (b + 3) * p.sa_col), w3 = __ldg(sw + (b + 3) * p.sw_k);
                 const uint64_t sc2 = pack2(sc, sc);
-                if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
-                if (++s == kPairStages) {
-                    s = 0;
-                    ph ^= 1u;
-                }
-                __syncwarp();
-                tc_after();
                 const uint32_t from = taddr + (uint32_t)(buf * 256);
                 uint64_t v[32];
+                if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
+                __syncwarp();
+                tc_after();
                 tmem_pairs(from, v);
 #pragma unroll
                 for (int c = 0; c < 32; ++c) fma2(acc[c], v[c], sc2);
@@ -257,6 +258,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
 #pragma unroll
                 for (int c = 0; c < 32; ++c) fma2(acc[32 + c], v[c], sc2);
+                if (++s == kPairStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
             if (m < p.M) {
 #pragma unroll
