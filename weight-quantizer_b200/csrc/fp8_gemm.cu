@@ -152,9 +152,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairCtlRegs));
-        if (warp == 0 && lane == 0) {
+        if (warp == 0) {
             // each CTA loads its 128 rows of a and its 128 columns of w; the
             // bytes count on the even CTA's barrier
+            const uint32_t full0 = in_cta(full(0), 0);
             int s = 0;
             uint32_t ph = 1;
             for (int t = first; t < tiles; t += pairs) {
@@ -163,19 +164,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int m0 = mt * kPairTile + rank * 128, n0 = nt * kPairTile + rank * 128;
                 for (int b = 0; b < p.blocks; ++b) {
                     if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
-                    const uint32_t f = in_cta(full(s), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
-                    const uint32_t dst = sbase + (uint32_t)(s * kPairStage);
-                    tma_box<2>(dst, &map_a, b * 128, m0, f);
-                    if constexpr (WT) tma_box<2>(dst + kOperandBytes, &map_w, n0, b * 128, f);
-                    else tma_box<2>(dst + kOperandBytes, &map_w, b * 128, n0, f);
+                    __syncwarp();
+                    if (elect_one()) {
+                        const uint32_t f = full0 + 8u * (uint32_t)s;
+                        const uint32_t dst = sbase + (uint32_t)(s * kPairStage);
+                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
+                        tma_box<2>(dst, &map_a, b * 128, m0, f);
+                        if constexpr (WT) tma_box<2>(dst + kOperandBytes, &map_w, n0, b * 128, f);
+                        else tma_box<2>(dst + kOperandBytes, &map_w, b * 128, n0, f);
+                    }
+                    __syncwarp();
                     if (++s == kPairStages) {
                         s = 0;
                         ph ^= 1u;
                     }
                 }
             }
-            // every copy this thread started has been read before the CTA goes
+            // every copy this warp started has been read before the CTA goes
             // (a stage that was never filled passes at once)
             for (int i = 0; i < kPairStages; ++i) {
                 if (!mbar_wait_bounded(done(s), ph)) atomicOr(p.fault, 1u);
