@@ -1,68 +1,528 @@
 // The weight gradient of a linear layer from the 8-bit checkpoint of its input.
 //
-//   dw[n, k] (+)= sum_m dy[m, n] c[m, k] s[m, k / 128]
+//   dw[n, k] (+)= sum_m dy[m, n] x^[m, k],   x^[m, k] = c[m, k] s[m, k / 128]
+//
+// The scale varies along the sum, so it cannot leave it: x^ enters the product as
+// an operand. With power-of-two scales (quantize_fp8's) code * scale is exact in
+// bf16, and dy is bf16 already, or is split into bf16 terms that add up to it (two
+// for fp16, three for fp32): every product is exact. Other scales' code * scale is
+// rounded to bf16 (half a step 2^-9 of each value), the operand type's only choice.
+//
+// Sums over 512 rows stay in tensor memory, then they are added to fp32 registers:
+// the tensor core's own additions cut off what they add, and over all rows of a
+// long batch that would grow to several steps of the result, all to one side.
 #include "fp8_types.cuh"
 #include "kernels.h"
+#include "launch.h"
+#include "tc_ptx.cuh"
 
 namespace wq {
 namespace {
 
-constexpr int kTile = 64;   // output tile, 4 x 4 values per thread
-constexpr int kStep = 32;   // rows of dy and x per shared-memory step
+// A pair of CTAs makes a 256 x 256 tile of dw with tcgen05.mma of cta_group::2 on
+// steps of 64 rows of dy and x. Both operands lie along the outer dimension in
+// memory (MN-major), so dy goes from memory to the MMA as it is: warp 0 loads
+// boxes of 64 rows x 64 columns. x^ is made by the eight working warps: 16 codes
+// per lane from L2 to registers, e4m3 -> fp16 -> fp32, times the row's scale, to
+// bf16 in the swizzled tile (reading the codes directly saves their way through
+// shared memory, whose bandwidth the MMA's operands already take half of). Warps
+// take turns by fours, two steps of time for each step of rows. The same warps add
+// the finished sums of 512 rows to their registers, three steps later, when the
+// MMAs are over anyway: a lane is a row of dw, a warp has 128 columns.
 
+constexpr int kTile = 256;
+constexpr int kStep = 64;                      // rows of dy and x per step
+constexpr int kSpan = 8;                       // steps whose sums stay in tensor memory
+constexpr int kPlaneBytes = kStep * 128 * 2;   // 64 rows x 128 columns in bf16: one CTA's operand of one step
+constexpr int kThreads = 384;
+constexpr int kLaunchRegs = 168, kCtlRegs = 56, kWorkRegs = 224;
+static_assert(kCtlRegs + 2 * kWorkRegs <= 3 * kLaunchRegs, "register split exceeds the launch's registers");
+
+// P terms of dy per step, then x^.
+template <int P>
+struct Smem {
+    static constexpr int STAGE = (P + 1) * kPlaneBytes;
+    static constexpr int STAGES = 200 * 1024 / STAGE;
+    static constexpr int BAR = STAGES * STAGE;
+    // full and done per stage; the odd CTA's x^ ready per stage; sums full[2], empty[2]
+    static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 4);
+    static constexpr int TOTAL = TMEM_SLOT + 16;
+    // steps of the next span made before a span's sums are read: its MMAs are over then
+    static constexpr int LAG = STAGES - 1 < 3 ? STAGES - 1 : 3;
+    static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
+};
+
+struct Params {
+    const uint8_t* codes;
+    int64_t ld;
+    const float* scales;
+    int64_t s_row, s_col;
+    void* out;
+    int out_type;
+    int64_t ldo;
+    int accumulate;
+    int M, N, K, steps;
+    int tiles_n, tiles_k, band;
+    bool wide_out;
+    unsigned int* fault;
+};
+
+// Tile t: bands of `band` column tiles of x; inside a band they run fastest, so
+// that the band's columns of x stay in L2 while dy streams by once.
+__device__ __forceinline__ void tile_of(int t, const Params& p, int& nt, int& kt) {
+    const int per = p.band * p.tiles_n;
+    const int b = t / per, in = t - b * per;
+    const int bw = min(p.band, p.tiles_k - b * p.band);
+    nt = in / bw;
+    kt = b * p.band + (in - nt * bw);
+}
+
+// Columns c .. c + 15 of a row of dw.
 template <typename O>
-__global__ void __launch_bounds__(256) fp8_wgrad_kernel(const Fp8WeightGrad g) {
-    __shared__ float ds[kStep][kTile + 4], xs[kStep][kTile + 4];
-    const int64_t n0 = (int64_t)blockIdx.y * kTile, k0 = (int64_t)blockIdx.x * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int64_t m0 = 0; m0 < g.M; m0 += kStep) {
-        for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-            const int r = i / kTile, c = i % kTile;
-            const int64_t m = m0 + r, n = n0 + c, k = k0 + c;
-            ds[r][c] = m < g.M && n < g.N ? load_any(g.dy, g.dy_type, m * g.ldy + n) : 0.0f;
-            xs[r][c] = m < g.M && k < g.K ? e4m3x2_values(g.a.codes[m * g.a.ld + k]).x *
-                                                g.a.scales[m * g.a.s_row + (k / kFp8Block) * g.a.s_col]
-                                          : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int r = 0; r < kStep; ++r) {
-            float dv[4], xv[4];
+__device__ __forceinline__ void put16(O* row, int64_t c, int64_t k, bool wide, const float (&v)[16], bool add) {
+    if (wide && c + 16 <= k) {
+        constexpr int PER = 4 / (int)sizeof(O);       // values in a word
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dv[i] = ds[r][ty * 4 + i];
-                xv[i] = xs[r][tx * 4 + i];
+        for (int i = 0; i < 16; i += 8 * PER) {
+            uint32_t w[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                O e[PER];
+                if (add) *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(row + c + i + q * PER);
+#pragma unroll
+                for (int j = 0; j < PER; ++j)
+                    e[j] = from_f32<O>(add ? to_f32<O>(e[j]) + v[i + q * PER + j] : v[i + q * PER + j]);
+                w[q] = *reinterpret_cast<const uint32_t*>(e);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(dv[i], xv[j], acc[i][j]);
+            st_32(row + c + i, w);
         }
-        __syncthreads();
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (c + i < k) row[c + i] = from_f32<O>(add ? to_f32<O>(row[c + i]) + v[i] : v[i]);
     }
+}
+
+template <int P>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy) {
+    using L = Smem<P>;
+    constexpr int NS = L::STAGES;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_addr(smem);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
+    const int rank = (int)cluster_rank();
+    auto bar = [&](int i) -> uint32_t { return sbase + L::BAR + 8u * (uint32_t)i; };
+    auto full = [&](int s) { return bar(s); };
+    auto done = [&](int s) { return bar(NS + s); };
+    auto made = [&](int s) { return bar(2 * NS + s); };
+    auto sums_full = [&](int b) { return bar(3 * NS + b); };
+    auto sums_empty = [&](int b) { return bar(3 * NS + 2 + b); };
+    launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            // the even CTA's: its loader's arrival with both CTAs' bytes of dy, its four
+            // warps that made x^, and one word that the odd CTA's x^ is there
+            mbar_init(full(s), 6);
+            mbar_init(done(s), 1);
+            mbar_init(made(s), 4);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(sums_full(b), 1);
+            mbar_init(sums_empty(b), 16);
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 1) tmem_alloc<2>(sbase + L::TMEM_SLOT, 512);
+    tc_before();
+    __syncthreads();
+    cluster_sync();
+    tc_after();
+    grid_wait();   // nothing above reads global memory
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_SLOT);
+    const int pairs = (int)gridDim.x >> 1, first = (int)blockIdx.x >> 1;
+    const int tiles = p.tiles_n * p.tiles_k;
+    const int mine = first < tiles ? (tiles - 1 - first) / pairs + 1 : 0;
+    bool faulted = false;
+    auto wait = [&](uint32_t b, uint32_t parity) {
+        if (!faulted && !mbar_wait_bounded(b, parity)) {
+            faulted = true;
+            atomicOr(p.fault, 1u);
+        }
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtlRegs));
+        if (warp == 0) {
+            const uint32_t full0 = in_cta(full(0), 0);
+            int s = 0;
+            uint32_t ph = 1;
+            for (int t = first; t < tiles; t += pairs) {
+                int nt, kt;
+                tile_of(t, p, nt, kt);
+                const int n0 = nt * kTile + rank * 128;
+                for (int i = 0; i < p.steps; ++i) {
+                    wait(done(s), ph);
+                    __syncwarp();
+                    if (elect_one()) {
+                        const uint32_t f = full0 + 8u * (uint32_t)s;
+                        const uint32_t dst = sbase + (uint32_t)(s * L::STAGE);
+                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * P * kPlaneBytes);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+                        for (int pl = 0; pl < P; ++pl) {
+                            // term pl of dy lies pl * M rows below the first; the rows
+                            // of another term that a last step reaches into meet x^ = 0
+                            const int y = pl * p.M + i * kStep;
+                            tma_box<2>(dst + pl * kPlaneBytes, &map_dy, n0, y, f);
+                            tma_box<2>(dst + pl * kPlaneBytes + kPlaneBytes / 2, &map_dy, n0 + 64, y, f);
+                        }
+                    }
+                    __syncwarp();
+                    if (++s == NS) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            // every copy this warp started has been read before the CTA goes
+            // (a stage that was never filled passes at once)
+            for (int i = 0; i < NS; ++i) {
+                if (!mbar_wait_bounded(done(s), ph)) atomicOr(p.fault, 1u);
+                if (++s == NS) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        } else if (warp == 1 && rank == 0) {
+            constexpr uint32_t idesc = mma_idesc(1, true, true, kTile, kTile);
+            const uint64_t desc0 = sw128_matrix(sbase, kPlaneBytes / 2);
+            int s = 0, buf = 0;
+            uint32_t ph = 0, reuse = 1;
+            for (int t = 0; t < mine; ++t) {
+                for (int i = 0; i < p.steps; ++i) {
+                    const int in = i % kSpan;
+                    if (in == 0) wait(sums_empty(buf), reuse);
+                    wait(full(s), ph);
+                    __syncwarp();
+                    tc_after();
+                    const bool last = in == kSpan - 1 || i == p.steps - 1;
+                    if (elect_one()) {
+                        const uint64_t d0 = desc0 + (uint64_t)(s * (L::STAGE >> 4));
+                        const uint64_t dx = d0 + (uint64_t)(P * (kPlaneBytes >> 4));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t n = n0 + ty * 4 + i, k = k0 + tx * 4 + j;
-            if (n < g.N && k < g.K) {
-                O* o = static_cast<O*>(g.out) + n * g.ldo + k;
-                *o = from_f32<O>(g.accumulate ? to_f32<O>(*o) + acc[i][j] : acc[i][j]);
+                        for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+                            for (int k = 0; k < kStep / 16; ++k)   // 16 rows of 128 bytes
+                                mma_bf16<2>(tmem + (uint32_t)(buf * 256), d0 + (uint64_t)(pl * (kPlaneBytes >> 4)) + 128u * k,
+                                            dx + 128u * k, idesc, in > 0 || pl > 0 || k > 0);
+                        mma_done<2>(done(s));
+                        if (last) mma_done<2>(sums_full(buf));
+                    }
+                    __syncwarp();
+                    if (last) {
+                        buf ^= 1;
+                        if (buf == 0) reuse ^= 1u;
+                    }
+                    if (++s == NS) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        } else if (warp == 2 && rank == 1) {
+            // passes the odd CTA's finished x^ on to the even CTA's barrier
+            const uint32_t full0 = in_cta(full(0), 0);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int64_t i = (int64_t)mine * p.steps; i > 0; --i) {
+                wait(made(s), ph);
+                __syncwarp();
+                if (lane == 0) arrive_in_cluster(full0 + 8u * (uint32_t)s);
+                if (++s == NS) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkRegs));
+        const int q = warp & 3, turn = (warp - 4) >> 2;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(turn * 128);
+        const uint32_t free0 = in_cta(sums_empty(0), 0);
+        // this lane's 16 codes of rows row0 + 4 * j of a step, j < 4
+        const int row0 = q * 16 + (lane >> 3), chunk = lane & 7;
+        uint4 code[4];
+        float scale[4];
+        // the next step's codes and scales of tile column kt, rows from m0
+        auto fetch = [&](int kt, int i) {
+            const int64_t k = (int64_t)kt * kTile + rank * 128 + chunk * 16;
+            const int64_t kb = min(k, (int64_t)p.K - 1) >> 7;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t m = (int64_t)i * kStep + row0 + 4 * j;
+                code[j] = make_uint4(0, 0, 0, 0);
+                scale[j] = 0.0f;
+                if (m < p.M && k < p.K) {
+                    const uint8_t* at = p.codes + m * p.ld + k;
+                    scale[j] = __ldg(p.scales + m * p.s_row + kb * p.s_col);
+                    if (k + 16 <= p.K) {
+                        code[j] = __ldg(reinterpret_cast<const uint4*>(at));
+                    } else {
+                        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int b = 0; b < 16; ++b)
+                            if (k + b < p.K) w[b >> 2] |= (uint32_t)at[b] << (8 * (b & 3));
+                        code[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        };
+        float acc[128];
+#pragma unroll
+        for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
+        // the codes of step i of tile t, or of the pair's tile that it falls into
+        auto fetch_from = [&](int t, int i) {
+            while (i >= p.steps && t < tiles) {
+                i -= p.steps;
+                t += pairs;
+            }
+            if (t < tiles) {
+                int nt, kt;
+                tile_of(t, p, nt, kt);
+                fetch(kt, i);
+            }
+        };
+        fetch_from(first, turn);
+        const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes) + (uint32_t)((chunk >> 2) * (kPlaneBytes / 2));
+        int t = first, i = 0;             // tile and step within it
+        int s = 0, buf = 0;
+        uint32_t ph = 1, sph = 0;
+        int64_t due = -1;                 // the step before which a finished span's sums are read
+        int due_t = 0;                    // its tile, and whether it is the tile's last
+        bool due_last = false;
+        for (int64_t g = 0;; ++g) {
+            if (g == due) {
+                wait(sums_full(buf), sph);
+                __syncwarp();
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) {
+                    uint64_t v[8];
+                    tmem_pairs(taddr + (uint32_t)(buf * 256 + c), v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 f = unpack2(v[k]);
+                        acc[c + 2 * k] += f.x;
+                        acc[c + 2 * k + 1] += f.y;
+                    }
+                }
+                tc_before();
+                __syncwarp();
+                if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
+                buf ^= 1;
+                if (buf == 0) sph ^= 1u;
+                if (due_last) {
+                    int nt, kt;
+                    tile_of(due_t, p, nt, kt);
+                    const int64_t n = (int64_t)nt * kTile + rank * 128 + q * 32 + lane;
+                    const int64_t k0 = (int64_t)kt * kTile + turn * 128;
+                    if (n < p.N) {
+#pragma unroll
+                        for (int c = 0; c < 128; c += 16) {
+                            float v[16];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
+                            if (p.out_type == kBf16)
+                                put16(static_cast<__nv_bfloat16*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v,
+                                      p.accumulate);
+                            else if (p.out_type == kF16)
+                                put16(static_cast<__half*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v, p.accumulate);
+                            else
+                                put16(static_cast<float*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v, p.accumulate);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
+                }
+            }
+            if (t >= tiles) break;
+            if ((int)(g & 1) == turn) {
+                wait(done(s), ph);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = row0 + 4 * j;
+                    // 16 codes are two 16-byte chunks of the swizzled row; lanes of the
+                    // upper 64 columns store theirs the other way round, so that eight
+                    // lanes' chunks fall on eight different groups of banks
+                    const uint32_t row = x_at + (uint32_t)(s * L::STAGE + r * 128);
+                    const int flip = chunk >> 2;
+                    const uint32_t w[4] = {code[j].x, code[j].y, code[j].z, code[j].w};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t two = flip ? w[2 - 2 * h + (b >> 1)] : w[2 * h + (b >> 1)];
+                            const float2 f = e4m3x2_values(two >> (16 * (b & 1)));
+                            const __nv_bfloat162 e = __floats2bfloat162_rn(f.x * scale[j], f.y * scale[j]);
+                            o[b] = *reinterpret_cast<const uint32_t*>(&e);
+                        }
+                        const uint32_t at = row + (uint32_t)(((((chunk & 3) << 1) + (h ^ flip)) ^ (r & 7)) << 4);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o[0]), "r"(o[1]),
+                                     "r"(o[2]), "r"(o[3])
+                                     : "memory");
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(rank == 0 ? full(s) : made(s));
+                fetch_from(t, i + 2);   // this warp's next step
+            }
+            if (++s == NS) {
+                s = 0;
+                ph ^= 1u;
+            }
+            if (i % kSpan == kSpan - 1 || i == p.steps - 1) {
+                due_t = t;
+                due_last = i == p.steps - 1;
+                // some steps later, but before the next span's last (if there is one)
+                const int next_i = due_last ? 0 : i + 1;
+                const bool more = !due_last || t + pairs < tiles;
+                const int len = min(kSpan, p.steps - next_i);
+                due = g + 1 + (more ? min(L::LAG, len - 1) : 0);
+            }
+            if (++i == p.steps) {
+                i = 0;
+                t += pairs;
+            }
+        }
+    }
+    tc_before();
+    __syncthreads();
+    cluster_sync();   // the pair's MMAs, arrivals and reads of tensor memory are over
+    tc_after();
+    if (warp == 1) tmem_free<2>(tmem, 512);
+}
+
+// dy as bf16 terms that add up to it (fp16: 2, fp32: 3), each [M, ld] below the
+// last: v cut off to bf16, then what is left (cut off, no term overflows and eight
+// bits go into each). A value that is not finite has it
+// in the first term and zeros below. bf16 input whose rows TMA cannot read (an odd
+// stride or address) is copied as its one term.
+template <typename T, int P>
+__global__ void __launch_bounds__(256) split_terms_kernel(const T* __restrict__ dy, int64_t M, int64_t N, int64_t ldy,
+                                                          __nv_bfloat16* __restrict__ out, int64_t ld) {
+    grid_wait();
+    launch_dependents();
+    const int64_t quads = ld / 4;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < M * quads;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        __nv_bfloat16 term[P][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v = n + k < N ? to_f32<T>(dy[m * ldy + n + k]) : 0.0f;
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl) {
+                term[pl][k] = __float2bfloat16_rz(v);
+                const float h = __bfloat162float(term[pl][k]);
+                v = fabsf(h) <= 3.402823466e38f ? v - h : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl)
+            *reinterpret_cast<uint2*>(out + (pl * M + m) * ld + n) = *reinterpret_cast<const uint2*>(term[pl]);
+    }
+}
+
+// dw = 0 where there are no rows (and nothing to add to).
+template <typename O>
+__global__ void zero_rows_kernel(O* out, int64_t N, int64_t K, int64_t ldo) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < N * K; i += (int64_t)gridDim.x * blockDim.x)
+        out[i / K * ldo + i % K] = from_f32<O>(0.0f);
+}
+
+int terms_of(int type) { return type == kBf16 ? 1 : (type == kF16 ? 2 : 3); }
+int64_t term_ld(int64_t N) { return (N + 7) / 8 * 8; }
+int bytes_of(int type) { return type == kF32 ? 4 : 2; }
+
+template <int P>
+cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
+    Params p;
+    p.codes = g.a.codes;
+    p.ld = g.a.ld;
+    p.scales = g.a.scales;
+    p.s_row = g.a.s_row;
+    p.s_col = g.a.s_col;
+    p.out = g.out;
+    p.out_type = g.out_type;
+    p.ldo = g.ldo;
+    p.accumulate = g.accumulate;
+    p.M = (int)g.M;
+    p.N = (int)g.N;
+    p.K = (int)g.K;
+    p.steps = (int)((g.M + kStep - 1) / kStep);
+    p.tiles_n = (int)((g.N + kTile - 1) / kTile);
+    p.tiles_k = (int)((g.K + kTile - 1) / kTile);
+    // a band's columns of x stay below 40 MB, well inside L2
+    int64_t band = ((int64_t)40 << 20) / (g.M * kTile);
+    band = band < 1 ? 1 : band;
+    const int64_t bands = (p.tiles_k + band - 1) / band;
+    p.band = (int)((p.tiles_k + bands - 1) / bands);
+    p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * bytes_of(g.out_type)) % 32 == 0;
+    p.fault = fault_word();
+    if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
+    CUtensorMap map;
+    if (!encode_rows(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, g.N, P * g.M, ld * 2, kStep))
+        return cudaErrorInvalidValue;
+    const size_t smem = (size_t)Smem<P>::TOTAL + 1024;
+    auto kern = fp8_wgrad_kernel<P>;
+    static std::atomic<int> ready[kMaxDevices];
+    cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kLaunchRegs, ready);
+    if (e != cudaSuccess) return e;
+    const int tiles = p.tiles_n * p.tiles_k;
+    const int pairs = sm_count() / 2;
+    LaunchConfig cfg(dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), kThreads, smem, s);
+    return cudaLaunchKernelEx(&cfg.c, kern, p, map);
+}
+
+template <typename T, int P>
+cudaError_t split_and_launch(const Fp8WeightGrad& g, void* workspace, cudaStream_t s) {
+    const int64_t ld = term_ld(g.N);
+    const int64_t want = (g.M * (ld / 4) + 255) / 256;
+    const int64_t most = (int64_t)sm_count() * 16;
+    LaunchConfig cfg(dim3((unsigned)(want < most ? want : most)), 256, 0, s);
+    cudaError_t e = cudaLaunchKernelEx(&cfg.c, split_terms_kernel<T, P>, static_cast<const T*>(g.dy), g.M, g.N, g.ldy,
+                                       static_cast<__nv_bfloat16*>(workspace), ld);
+    if (e != cudaSuccess) return e;
+    return launch_p<P>(g, workspace, ld, s);
 }
 
 }  // namespace
 
-size_t fp8_weight_grad_workspace_bytes(int64_t, int64_t, int64_t, int) { return 0; }
+size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t, int dy_type) {
+    return (size_t)terms_of(dy_type) * (size_t)M * (size_t)term_ld(N) * 2;
+}
 
-cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void*, cudaStream_t s) {
-    const dim3 grid((unsigned)((g.K + kTile - 1) / kTile), (unsigned)((g.N + kTile - 1) / kTile));
-    if (g.out_type == kF16) fp8_wgrad_kernel<__half><<<grid, 256, 0, s>>>(g);
-    else if (g.out_type == kBf16) fp8_wgrad_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
-    else fp8_wgrad_kernel<float><<<grid, 256, 0, s>>>(g);
-    return cudaGetLastError();
+cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cudaStream_t s) {
+    if (g.M == 0) {
+        if (g.accumulate) return cudaSuccess;
+        const int64_t n = (g.N * g.K + 255) / 256;
+        const unsigned grid = (unsigned)(n < 65536 ? n : 65536);
+        if (g.out_type == kF16) zero_rows_kernel<<<grid, 256, 0, s>>>(static_cast<__half*>(g.out), g.N, g.K, g.ldo);
+        else if (g.out_type == kBf16)
+            zero_rows_kernel<<<grid, 256, 0, s>>>(static_cast<__nv_bfloat16*>(g.out), g.N, g.K, g.ldo);
+        else zero_rows_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(g.out), g.N, g.K, g.ldo);
+        return cudaGetLastError();
+    }
+    if (g.dy_type == kF32) return split_and_launch<float, 3>(g, workspace, s);
+    if (g.dy_type == kF16) return split_and_launch<__half, 2>(g, workspace, s);
+    if ((reinterpret_cast<uintptr_t>(g.dy) & 15) != 0 || (g.ldy * 2) % 16 != 0)
+        return split_and_launch<__nv_bfloat16, 1>(g, workspace, s);
+    return launch_p<1>(g, g.dy, g.ldy, s);
 }
 
 }  // namespace wq
