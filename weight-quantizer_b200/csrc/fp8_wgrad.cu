@@ -22,21 +22,21 @@ namespace {
 // A pair of CTAs makes a 256 x 256 tile of dw with tcgen05.mma of cta_group::2 on
 // steps of 64 rows of dy and x. Both operands lie along the outer dimension in
 // memory (MN-major), so dy goes from memory to the MMA as it is: warp 0 loads
-// boxes of 64 rows x 64 columns. x^ is made by the eight working warps: 16 codes
-// per lane from L2 to registers, e4m3 -> fp16 -> fp32, times the row's scale, to
-// bf16 in the swizzled tile (reading the codes directly saves their way through
-// shared memory, whose bandwidth the MMA's operands already take half of). Warps
-// take turns by fours, two steps of time for each step of rows. The same warps add
-// the finished sums of 512 rows to their registers, three steps later, when the
-// MMAs are over anyway: a lane is a row of dw, a warp has 128 columns.
+// boxes of 64 rows x 64 columns. x^ is made by eight warps (4-11): 16 codes per lane
+// from L2 to registers, e4m3 -> fp16 -> fp32, times the row's scale, to bf16 in the
+// swizzled tile (reading the codes directly saves their way through shared memory,
+// whose bandwidth the MMA's operands already take half of). They take turns by
+// fours: each step of rows has two steps of time. Eight more (12-19) add the
+// finished sums of 512 rows to their registers: a lane is a row of dw, a warp has
+// 128 columns.
 
 constexpr int kTile = 256;
 constexpr int kStep = 64;                      // rows of dy and x per step
 constexpr int kSpan = 8;                       // steps whose sums stay in tensor memory
 constexpr int kPlaneBytes = kStep * 128 * 2;   // 64 rows x 128 columns in bf16: one CTA's operand of one step
-constexpr int kThreads = 384;
-constexpr int kLaunchRegs = 168, kCtlRegs = 56, kWorkRegs = 224;
-static_assert(kCtlRegs + 2 * kWorkRegs <= 3 * kLaunchRegs, "register split exceeds the launch's registers");
+constexpr int kThreads = 640;
+constexpr int kLaunchRegs = 96, kCtlRegs = 40, kMakeRegs = 56, kSumRegs = 160;
+static_assert(kCtlRegs + 2 * kMakeRegs + 2 * kSumRegs <= 5 * kLaunchRegs, "register split exceeds the launch's registers");
 
 // P terms of dy per step, then x^.
 template <int P>
@@ -47,8 +47,6 @@ struct Smem {
     // full and done per stage; the odd CTA's x^ ready per stage; sums full[2], empty[2]
     static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 4);
     static constexpr int TOTAL = TMEM_SLOT + 16;
-    // steps of the next span made before a span's sums are read: its MMAs are over then
-    static constexpr int LAG = STAGES - 1 < 3 ? STAGES - 1 : 3;
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
 };
 
@@ -58,7 +56,6 @@ struct Params {
     const float* scales;
     int64_t s_row, s_col;
     void* out;
-    int out_type;
     int64_t ldo;
     int accumulate;
     int M, N, K, steps;
@@ -103,7 +100,7 @@ __device__ __forceinline__ void put16(O* row, int64_t c, int64_t k, bool wide, c
     }
 }
 
-template <int P>
+template <int P, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy) {
     using L = Smem<P>;
@@ -246,108 +243,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkRegs));
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMakeRegs));
         const int q = warp & 3, turn = (warp - 4) >> 2;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(turn * 128);
-        const uint32_t free0 = in_cta(sums_empty(0), 0);
         // this lane's 16 codes of rows row0 + 4 * j of a step, j < 4
         const int row0 = q * 16 + (lane >> 3), chunk = lane & 7;
         uint4 code[4];
         float scale[4];
-        // the next step's codes and scales of tile column kt, rows from m0
-        auto fetch = [&](int kt, int i) {
-            const int64_t k = (int64_t)kt * kTile + rank * 128 + chunk * 16;
-            const int64_t kb = min(k, (int64_t)p.K - 1) >> 7;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = (int64_t)i * kStep + row0 + 4 * j;
-                code[j] = make_uint4(0, 0, 0, 0);
-                scale[j] = 0.0f;
-                if (m < p.M && k < p.K) {
-                    const uint8_t* at = p.codes + m * p.ld + k;
-                    scale[j] = __ldg(p.scales + m * p.s_row + kb * p.s_col);
-                    if (k + 16 <= p.K) {
-                        code[j] = __ldg(reinterpret_cast<const uint4*>(at));
-                    } else {
-                        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int b = 0; b < 16; ++b)
-                            if (k + b < p.K) w[b >> 2] |= (uint32_t)at[b] << (8 * (b & 3));
-                        code[j] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
+        // the step whose codes are fetched next: of tile ft, rows from fi * kStep, this
+        // lane's first row and 16 columns at code_at
+        int ft = first, fi = turn;
+        const uint8_t* code_at = nullptr;
+        const float* scale_at = nullptr;
+        int wide_k = 0;                   // all of the CTA's 128 columns of x exist
+        int left_k = 0;                   // columns from this lane's 16 on
+        auto seek = [&]() {               // after a change of tile
+            while (fi >= p.steps && ft < tiles) {
+                fi -= p.steps;
+                ft += pairs;
             }
+            if (ft >= tiles) return;
+            int nt, kt;
+            tile_of(ft, p, nt, kt);
+            const int k0 = kt * kTile + rank * 128;
+            const int64_t m = (int64_t)fi * kStep + row0;
+            wide_k = k0 + 128 <= p.K;
+            left_k = p.K - (k0 + chunk * 16);
+            code_at = p.codes + m * p.ld + k0 + chunk * 16;
+            scale_at = p.scales + m * p.s_row + (min(k0, p.K - 1) >> 7) * p.s_col;
         };
-        float acc[128];
+        auto fetch = [&]() {
+            if (ft >= tiles) return;
+            if (wide_k && (fi + 1) * kStep <= p.M) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
-        // the codes of step i of tile t, or of the pair's tile that it falls into
-        auto fetch_from = [&](int t, int i) {
-            while (i >= p.steps && t < tiles) {
-                i -= p.steps;
-                t += pairs;
-            }
-            if (t < tiles) {
-                int nt, kt;
-                tile_of(t, p, nt, kt);
-                fetch(kt, i);
-            }
-        };
-        fetch_from(first, turn);
-        const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes) + (uint32_t)((chunk >> 2) * (kPlaneBytes / 2));
-        int t = first, i = 0;             // tile and step within it
-        int s = 0, buf = 0;
-        uint32_t ph = 1, sph = 0;
-        int64_t due = -1;                 // the step before which a finished span's sums are read
-        int due_t = 0;                    // its tile, and whether it is the tile's last
-        bool due_last = false;
-        for (int64_t g = 0;; ++g) {
-            if (g == due) {
-                wait(sums_full(buf), sph);
-                __syncwarp();
-                tc_after();
-#pragma unroll
-                for (int c = 0; c < 128; c += 16) {
-                    uint64_t v[8];
-                    tmem_pairs(taddr + (uint32_t)(buf * 256 + c), v);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float2 f = unpack2(v[k]);
-                        acc[c + 2 * k] += f.x;
-                        acc[c + 2 * k + 1] += f.y;
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    code[j] = __ldg(reinterpret_cast<const uint4*>(code_at + 4 * j * p.ld));
+                    scale[j] = __ldg(scale_at + 4 * j * p.s_row);
                 }
-                tc_before();
-                __syncwarp();
-                if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
-                buf ^= 1;
-                if (buf == 0) sph ^= 1u;
-                if (due_last) {
-                    int nt, kt;
-                    tile_of(due_t, p, nt, kt);
-                    const int64_t n = (int64_t)nt * kTile + rank * 128 + q * 32 + lane;
-                    const int64_t k0 = (int64_t)kt * kTile + turn * 128;
-                    if (n < p.N) {
+            } else {
 #pragma unroll
-                        for (int c = 0; c < 128; c += 16) {
-                            float v[16];
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
-                            if (p.out_type == kBf16)
-                                put16(static_cast<__nv_bfloat16*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v,
-                                      p.accumulate);
-                            else if (p.out_type == kF16)
-                                put16(static_cast<__half*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v, p.accumulate);
-                            else
-                                put16(static_cast<float*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v, p.accumulate);
+                for (int j = 0; j < 4; ++j) {
+                    code[j] = make_uint4(0, 0, 0, 0);
+                    scale[j] = 0.0f;
+                    if (fi * kStep + row0 + 4 * j < p.M && left_k > 0) {
+                        const uint8_t* at = code_at + 4 * j * p.ld;
+                        scale[j] = __ldg(scale_at + 4 * j * p.s_row);
+                        if (left_k >= 16) {
+                            code[j] = __ldg(reinterpret_cast<const uint4*>(at));
+                        } else {
+                            uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+                            for (int b = 0; b < left_k; ++b) {
+                                if (b < 8) lo |= (uint64_t)at[b] << (8 * b);
+                                else hi |= (uint64_t)at[b] << (8 * (b - 8));
+                            }
+                            code[j] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
                         }
                     }
-#pragma unroll
-                    for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
                 }
             }
-            if (t >= tiles) break;
+            fi += 2;
+            code_at += 2 * kStep * p.ld;
+            scale_at += 2 * kStep * p.s_row;
+            if (fi >= p.steps) seek();
+        };
+        seek();
+        fetch();
+        const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes) + (uint32_t)((chunk >> 2) * (kPlaneBytes / 2));
+        int s = 0;
+        uint32_t ph = 1;
+        const int64_t steps = (int64_t)mine * p.steps;
+        for (int64_t g = 0; g < steps; ++g) {
             if ((int)(g & 1) == turn) {
                 wait(done(s), ph);
                 __syncwarp();
@@ -379,24 +345,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(rank == 0 ? full(s) : made(s));
-                fetch_from(t, i + 2);   // this warp's next step
+                fetch();   // this warp's next step
             }
             if (++s == NS) {
                 s = 0;
                 ph ^= 1u;
             }
-            if (i % kSpan == kSpan - 1 || i == p.steps - 1) {
-                due_t = t;
-                due_last = i == p.steps - 1;
-                // some steps later, but before the next span's last (if there is one)
-                const int next_i = due_last ? 0 : i + 1;
-                const bool more = !due_last || t + pairs < tiles;
-                const int len = min(kSpan, p.steps - next_i);
-                due = g + 1 + (more ? min(L::LAG, len - 1) : 0);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+        const int q = warp & 3, half = (warp - 12) >> 2;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t free0 = in_cta(sums_empty(0), 0);
+        int buf = 0;
+        uint32_t ph = 0;
+        for (int t = first; t < tiles; t += pairs) {
+            float acc[128];
+#pragma unroll
+            for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
+            for (int i = 0; i < p.steps; i += kSpan) {
+                wait(sums_full(buf), ph);
+                __syncwarp();
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) {
+                    uint64_t v[8];
+                    tmem_pairs(taddr + (uint32_t)(buf * 256 + c), v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 f = unpack2(v[k]);
+                        acc[c + 2 * k] += f.x;
+                        acc[c + 2 * k + 1] += f.y;
+                    }
+                }
+                tc_before();
+                __syncwarp();
+                if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
+                buf ^= 1;
+                if (buf == 0) ph ^= 1u;
             }
-            if (++i == p.steps) {
-                i = 0;
-                t += pairs;
+            int nt, kt;
+            tile_of(t, p, nt, kt);
+            const int64_t n = (int64_t)nt * kTile + rank * 128 + q * 32 + lane;
+            const int64_t k0 = (int64_t)kt * kTile + half * 128;
+            if (n < p.N) {
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) {
+                    float v[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
+                    put16(static_cast<O*>(p.out) + n * p.ldo, k0 + c, p.K, p.wide_out, v, p.accumulate);
+                }
             }
         }
     }
@@ -449,8 +448,8 @@ int terms_of(int type) { return type == kBf16 ? 1 : (type == kF16 ? 2 : 3); }
 int64_t term_ld(int64_t N) { return (N + 7) / 8 * 8; }
 int bytes_of(int type) { return type == kF32 ? 4 : 2; }
 
-template <int P>
-cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
+template <int P, typename O>
+cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
     Params p;
     p.codes = g.a.codes;
     p.ld = g.a.ld;
@@ -458,7 +457,6 @@ cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStr
     p.s_row = g.a.s_row;
     p.s_col = g.a.s_col;
     p.out = g.out;
-    p.out_type = g.out_type;
     p.ldo = g.ldo;
     p.accumulate = g.accumulate;
     p.M = (int)g.M;
@@ -479,7 +477,7 @@ cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStr
     if (!encode_rows(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, g.N, P * g.M, ld * 2, kStep))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)Smem<P>::TOTAL + 1024;
-    auto kern = fp8_wgrad_kernel<P>;
+    auto kern = fp8_wgrad_kernel<P, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kLaunchRegs, ready);
     if (e != cudaSuccess) return e;
@@ -487,6 +485,13 @@ cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStr
     const int pairs = sm_count() / 2;
     LaunchConfig cfg(dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), kThreads, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, map);
+}
+
+template <int P>
+cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
+    if (g.out_type == kF16) return launch_po<P, __half>(g, dy, ld, s);
+    if (g.out_type == kBf16) return launch_po<P, __nv_bfloat16>(g, dy, ld, s);
+    return launch_po<P, float>(g, dy, ld, s);
 }
 
 template <typename T, int P>
