@@ -22,13 +22,14 @@ namespace {
 // A pair of CTAs makes a 256 x 256 tile of dw with tcgen05.mma of cta_group::2 on
 // steps of 64 rows of dy and x. Both operands lie along the outer dimension in
 // memory (MN-major), so dy goes from memory to the MMA as it is: warp 0 loads
-// boxes of 64 rows x 64 columns. x^ is made by eight warps (4-11): 16 codes per lane
-// from L2 to registers, e4m3 -> fp16 -> fp32, times the row's scale, to bf16 in the
-// swizzled tile (reading the codes directly saves their way through shared memory,
-// whose bandwidth the MMA's operands already take half of). They take turns by
-// fours: each step of rows has two steps of time. Eight more (12-19) add the
-// finished sums of 512 rows to their registers: a lane is a row of dw, a warp has
-// 128 columns.
+// boxes of 64 rows x 64 columns. x^ is made by eight warps (4-11), which take turns
+// by fours, so that each step of rows has two steps of time: every lane copies its
+// own 16 codes of four rows into shared memory three turns ahead (asynchronous
+// copies, which also end at x's edges), then e4m3 -> fp16 -> fp32, times the row's
+// scale, to bf16 in the swizzled tile. (Codes loaded one turn ahead into registers
+// arrived too late: 1050 cycles for a step whose MMAs take 512.) Eight more warps
+// (12-19) add the finished sums of 512 rows to their registers: a lane is a row of
+// dw, a warp has 128 columns.
 
 constexpr int kTile = 256;
 constexpr int kStep = 64;                      // rows of dy and x per step
@@ -38,12 +39,19 @@ constexpr int kThreads = 640;
 constexpr int kLaunchRegs = 96, kCtlRegs = 40, kMakeRegs = 56, kSumRegs = 160;
 static_assert(kCtlRegs + 2 * kMakeRegs + 2 * kSumRegs <= 5 * kLaunchRegs, "register split exceeds the launch's registers");
 
-// P terms of dy per step, then x^.
+// Codes on their way: for each of the eight warps kAhead + 1 turns of 32 lanes x 4
+// rows x 16 codes and 16 rows' scales.
+constexpr int kAhead = 3;
+constexpr int kTurnBytes = 32 * 4 * 16 + 16 * 4;
+constexpr int kCodesBytes = 8 * (kAhead + 1) * kTurnBytes;
+
+// P terms of dy per step, then x^; the codes on their way.
 template <int P>
 struct Smem {
     static constexpr int STAGE = (P + 1) * kPlaneBytes;
-    static constexpr int STAGES = 200 * 1024 / STAGE;
-    static constexpr int BAR = STAGES * STAGE;
+    static constexpr int STAGES = (224 * 1024 - kCodesBytes) / STAGE;
+    static constexpr int CODES = STAGES * STAGE;
+    static constexpr int BAR = CODES + kCodesBytes;
     // full and done per stage; the odd CTA's x^ ready per stage; sums full[2], empty[2]
     static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 4);
     static constexpr int TOTAL = TMEM_SLOT + 16;
@@ -248,15 +256,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int q = warp & 3, turn = (warp - 4) >> 2;
         // this lane's 16 codes of rows row0 + 4 * j of a step, j < 4
         const int row0 = q * 16 + (lane >> 3), chunk = lane & 7;
-        uint4 code[4];
-        float scale[4];
-        // the step whose codes are fetched next: of tile ft, rows from fi * kStep, this
-        // lane's first row and 16 columns at code_at
+        // the turn that is copied next: step fi of tile ft; this lane's first row and
+        // 16 columns at code_at, the scale of row 16 q + lane % 16 at scale_at
         int ft = first, fi = turn;
         const uint8_t* code_at = nullptr;
         const float* scale_at = nullptr;
-        int wide_k = 0;                   // all of the CTA's 128 columns of x exist
-        int left_k = 0;                   // columns from this lane's 16 on
+        int left_k = 0;                   // columns of x from this lane's 16 on
         auto seek = [&]() {               // after a change of tile
             while (fi >= p.steps && ft < tiles) {
                 fi -= p.steps;
@@ -266,55 +271,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             int nt, kt;
             tile_of(ft, p, nt, kt);
             const int k0 = kt * kTile + rank * 128;
-            const int64_t m = (int64_t)fi * kStep + row0;
-            wide_k = k0 + 128 <= p.K;
             left_k = p.K - (k0 + chunk * 16);
-            code_at = p.codes + m * p.ld + k0 + chunk * 16;
-            scale_at = p.scales + m * p.s_row + (min(k0, p.K - 1) >> 7) * p.s_col;
+            code_at = p.codes + ((int64_t)fi * kStep + row0) * p.ld + k0 + chunk * 16;
+            scale_at = p.scales + ((int64_t)fi * kStep + q * 16 + (lane & 15)) * p.s_row + (min(k0, p.K - 1) >> 7) * p.s_col;
         };
-        auto fetch = [&]() {
-            if (ft >= tiles) return;
-            if (wide_k && (fi + 1) * kStep <= p.M) {
+        const uint32_t ring = sbase + (uint32_t)(L::CODES + (warp - 4) * (kAhead + 1) * kTurnBytes);
+        int in = 0, out = 0;              // ring positions
+        auto copy = [&]() {
+            if (ft < tiles) {
+                const int rows = p.M - fi * kStep;
+                const uint32_t to = ring + (uint32_t)(in * kTurnBytes);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    code[j] = __ldg(reinterpret_cast<const uint4*>(code_at + 4 * j * p.ld));
-                    scale[j] = __ldg(scale_at + 4 * j * p.s_row);
+                    // what lies outside x reads as 0 (and its address is not used)
+                    const int n = row0 + 4 * j < rows ? max(0, min(16, left_k)) : 0;
+                    cp_async16_n(to + (uint32_t)((j * 32 + lane) * 16), n > 0 ? code_at + 4 * j * p.ld : p.codes, n);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    code[j] = make_uint4(0, 0, 0, 0);
-                    scale[j] = 0.0f;
-                    if (fi * kStep + row0 + 4 * j < p.M && left_k > 0) {
-                        const uint8_t* at = code_at + 4 * j * p.ld;
-                        scale[j] = __ldg(scale_at + 4 * j * p.s_row);
-                        if (left_k >= 16) {
-                            code[j] = __ldg(reinterpret_cast<const uint4*>(at));
-                        } else {
-                            uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-                            for (int b = 0; b < left_k; ++b) {
-                                if (b < 8) lo |= (uint64_t)at[b] << (8 * b);
-                                else hi |= (uint64_t)at[b] << (8 * (b - 8));
-                            }
-                            code[j] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
-                        }
-                    }
-                }
+                const bool some = q * 16 + (lane & 15) < rows;
+                if (lane < 16) cp_async4_s(to + 32 * 4 * 16 + lane * 4, some ? scale_at : p.scales, some);
+                fi += 2;
+                code_at += 2 * kStep * p.ld;
+                scale_at += 2 * kStep * p.s_row;
+                if (fi >= p.steps) seek();
             }
-            fi += 2;
-            code_at += 2 * kStep * p.ld;
-            scale_at += 2 * kStep * p.s_row;
-            if (fi >= p.steps) seek();
+            cp_async_commit();
+            in = in == kAhead ? 0 : in + 1;
         };
         seek();
-        fetch();
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) copy();
         const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes) + (uint32_t)((chunk >> 2) * (kPlaneBytes / 2));
         int s = 0;
         uint32_t ph = 1;
         const int64_t steps = (int64_t)mine * p.steps;
         for (int64_t g = 0; g < steps; ++g) {
             if ((int)(g & 1) == turn) {
+                copy();
+                cp_async_wait<kAhead>();
+                __syncwarp();             // the scales were copied by other lanes
+                const unsigned char* from = smem + (ring - sbase) + out * kTurnBytes;
+                out = out == kAhead ? 0 : out + 1;
+                uint4 code[4];
+                float scale[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    code[j] = *reinterpret_cast<const uint4*>(from + (j * 32 + lane) * 16);
+                    scale[j] = *reinterpret_cast<const float*>(from + 32 * 4 * 16 + ((lane >> 3) + 4 * j) * 4);
+                }
                 wait(done(s), ph);
                 __syncwarp();
 #pragma unroll
@@ -345,7 +348,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(rank == 0 ? full(s) : made(s));
-                fetch();   // this warp's next step
             }
             if (++s == NS) {
                 s = 0;

@@ -255,6 +255,12 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             : "memory");
 }
 
+// Asynchronous copy of n <= 16 bytes into 16 bytes of shared memory, the rest zeros
+// (n = 0 reads nothing).
+__device__ __forceinline__ void cp_async16_n(uint32_t dst, const void* src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
 // ---- CTA pairs -----------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
