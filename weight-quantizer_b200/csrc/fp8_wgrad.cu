@@ -23,11 +23,11 @@ namespace {
 // steps of 64 rows of dy and x. Both operands lie along the outer dimension in
 // memory (MN-major), so dy goes from memory to the MMA as it is: warp 0 loads
 // boxes of 64 rows x 64 columns. x^ is made by eight warps (4-11), which take turns
-// by fours, so that each step of rows has two steps of time: every lane copies its
-// own 16 codes of four rows into shared memory three turns ahead (asynchronous
-// copies, which also end at x's edges), then e4m3 -> fp16 -> fp32, times the row's
-// scale, to bf16 in the swizzled tile. (Codes loaded one turn ahead into registers
-// arrived too late: 1050 cycles for a step whose MMAs take 512.) Eight more warps
+// by fours, so that each step of rows has two steps of time: codes (TMA) and scales
+// (asynchronous copies) come into shared memory some steps ahead by warp 3, then
+// e4m3 -> fp16 -> fp32, times the row's scale, to bf16 in the swizzled tile; a lane
+// takes eight codes of each 64 columns, which are one 16-byte chunk of that tile, so
+// that eight lanes fill a row without bank conflicts. Eight more warps
 // (12-19) add the finished sums of 512 rows to their registers: a lane is a row of
 // dw, a warp has 128 columns.
 
@@ -39,28 +39,27 @@ constexpr int kThreads = 640;
 constexpr int kLaunchRegs = 96, kCtlRegs = 40, kMakeRegs = 56, kSumRegs = 160;
 static_assert(kCtlRegs + 2 * kMakeRegs + 2 * kSumRegs <= 5 * kLaunchRegs, "register split exceeds the launch's registers");
 
-// Codes on their way: for each of the eight warps kAhead + 1 turns of 32 lanes x 4
-// rows x 16 codes and 16 rows' scales.
-constexpr int kAhead = 3;
-constexpr int kTurnBytes = 32 * 4 * 16 + 16 * 4;
-constexpr int kCodesBytes = 8 * (kAhead + 1) * kTurnBytes;
+// Codes on their way: 64 rows of 128 codes (128-byte swizzle) and their scales.
+constexpr int kAhead = 6;
+constexpr int kCodesBytes = kStep * 128;
 
-// P terms of dy per step, then x^; the codes on their way.
+// P terms of dy per step, then x^; the codes on their way, their scales.
 template <int P>
 struct Smem {
     static constexpr int STAGE = (P + 1) * kPlaneBytes;
-    static constexpr int STAGES = (224 * 1024 - kCodesBytes) / STAGE;
+    static constexpr int STAGES = (222 * 1024 - kAhead * (kCodesBytes + kStep * 4)) / STAGE;
     static constexpr int CODES = STAGES * STAGE;
-    static constexpr int BAR = CODES + kCodesBytes;
-    // full and done per stage; the odd CTA's x^ ready per stage; sums full[2], empty[2]
-    static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 4);
+    static constexpr int SCALES = CODES + kAhead * kCodesBytes;
+    static constexpr int BAR = SCALES + kAhead * kStep * 4;
+    // full and done per stage; the odd CTA's x^ ready per stage; codes there and read;
+    // sums full[2], empty[2]
+    static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 2 * kAhead + 4);
     static constexpr int TOTAL = TMEM_SLOT + 16;
+    static_assert(STAGES >= 2, "the MMAs of one step run while the next is made");
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
 };
 
 struct Params {
-    const uint8_t* codes;
-    int64_t ld;
     const float* scales;
     int64_t s_row, s_col;
     void* out;
@@ -110,7 +109,8 @@ __device__ __forceinline__ void put16(O* row, int64_t c, int64_t k, bool wide, c
 
 template <int P, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy) {
+    fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy,
+                     const __grid_constant__ CUtensorMap map_x) {
     using L = Smem<P>;
     constexpr int NS = L::STAGES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -123,8 +123,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto full = [&](int s) { return bar(s); };
     auto done = [&](int s) { return bar(NS + s); };
     auto made = [&](int s) { return bar(2 * NS + s); };
-    auto sums_full = [&](int b) { return bar(3 * NS + b); };
-    auto sums_empty = [&](int b) { return bar(3 * NS + 2 + b); };
+    auto codes_full = [&](int a) { return bar(3 * NS + a); };
+    auto codes_read = [&](int a) { return bar(3 * NS + kAhead + a); };
+    auto sums_full = [&](int b) { return bar(3 * NS + 2 * kAhead + b); };
+    auto sums_empty = [&](int b) { return bar(3 * NS + 2 * kAhead + 2 + b); };
     launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
@@ -133,6 +135,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(full(s), 6);
             mbar_init(done(s), 1);
             mbar_init(made(s), 4);
+        }
+        for (int a = 0; a < kAhead; ++a) {
+            mbar_init(codes_full(a), 33);   // the codes' bytes, and every lane's copies of scales
+            mbar_init(codes_read(a), 4);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(sums_full(b), 1);
@@ -250,104 +256,106 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     ph ^= 1u;
                 }
             }
+        } else if (warp == 3) {
+            // each CTA's 128 columns of codes, and its rows' scales of their block
+            int a = 0;
+            uint32_t ph = 1;
+            for (int t = first; t < tiles; t += pairs) {
+                int nt, kt;
+                tile_of(t, p, nt, kt);
+                const int k0 = kt * kTile + rank * 128;
+                const float* sc = p.scales + (min(k0, p.K - 1) >> 7) * p.s_col;
+                for (int i = 0; i < p.steps; ++i) {
+                    wait(codes_read(a), ph);
+                    __syncwarp();
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(codes_full(a), kCodesBytes);
+                        tma_box<1>(sbase + (uint32_t)(L::CODES + a * kCodesBytes), &map_x, k0, i * kStep, codes_full(a));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int64_t m = (int64_t)i * kStep + h * 32 + lane;   // (rows beyond the last: scale 0)
+                        cp_async4_s(sbase + (uint32_t)(L::SCALES + (a * kStep + h * 32 + lane) * 4),
+                                    m < p.M ? sc + m * p.s_row : p.scales, m < p.M);
+                    }
+                    cp_async_arrive(codes_full(a));
+                    if (++a == kAhead) {
+                        a = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            for (int i = 0; i < kAhead; ++i) {   // as warp 0 does
+                if (!mbar_wait_bounded(codes_read(a), ph)) atomicOr(p.fault, 1u);
+                if (++a == kAhead) {
+                    a = 0;
+                    ph ^= 1u;
+                }
+            }
         }
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMakeRegs));
         const int q = warp & 3, turn = (warp - 4) >> 2;
-        // this lane's 16 codes of rows row0 + 4 * j of a step, j < 4
-        const int row0 = q * 16 + (lane >> 3), chunk = lane & 7;
-        // the turn that is copied next: step fi of tile ft; this lane's first row and
-        // 16 columns at code_at, the scale of row 16 q + lane % 16 at scale_at
-        int ft = first, fi = turn;
-        const uint8_t* code_at = nullptr;
-        const float* scale_at = nullptr;
-        int left_k = 0;                   // columns of x from this lane's 16 on
-        auto seek = [&]() {               // after a change of tile
-            while (fi >= p.steps && ft < tiles) {
-                fi -= p.steps;
-                ft += pairs;
-            }
-            if (ft >= tiles) return;
-            int nt, kt;
-            tile_of(ft, p, nt, kt);
-            const int k0 = kt * kTile + rank * 128;
-            left_k = p.K - (k0 + chunk * 16);
-            code_at = p.codes + ((int64_t)fi * kStep + row0) * p.ld + k0 + chunk * 16;
-            scale_at = p.scales + ((int64_t)fi * kStep + q * 16 + (lane & 15)) * p.s_row + (min(k0, p.K - 1) >> 7) * p.s_col;
-        };
-        const uint32_t ring = sbase + (uint32_t)(L::CODES + (warp - 4) * (kAhead + 1) * kTurnBytes);
-        int in = 0, out = 0;              // ring positions
-        auto copy = [&]() {
-            if (ft < tiles) {
-                const int rows = p.M - fi * kStep;
-                const uint32_t to = ring + (uint32_t)(in * kTurnBytes);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // what lies outside x reads as 0 (and its address is not used)
-                    const int n = row0 + 4 * j < rows ? max(0, min(16, left_k)) : 0;
-                    cp_async16_n(to + (uint32_t)((j * 32 + lane) * 16), n > 0 ? code_at + 4 * j * p.ld : p.codes, n);
-                }
-                const bool some = q * 16 + (lane & 15) < rows;
-                if (lane < 16) cp_async4_s(to + 32 * 4 * 16 + lane * 4, some ? scale_at : p.scales, some);
-                fi += 2;
-                code_at += 2 * kStep * p.ld;
-                scale_at += 2 * kStep * p.s_row;
-                if (fi >= p.steps) seek();
-            }
-            cp_async_commit();
-            in = in == kAhead ? 0 : in + 1;
-        };
-        seek();
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) copy();
-        const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes) + (uint32_t)((chunk >> 2) * (kPlaneBytes / 2));
-        int s = 0;
-        uint32_t ph = 1;
+        // this lane's rows row_of(j) of a step, j < 4, and its chunk of eight codes. (Two
+        // rows that a half-warp reads at once are four apart: their chunks lie in
+        // different halves of the swizzled 128 bytes.)
+        const int sub = lane >> 3, chunk = lane & 7;
+        const int row0 = q * 16 + (sub >> 1) + 4 * (sub & 1);
+        auto row_of = [&](int j) { return row0 + 2 * (j & 1) + 8 * (j >> 1); };
+        const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes);
+        int s = 0, a = 0;
+        uint32_t ph = 1, aph = 0;
         const int64_t steps = (int64_t)mine * p.steps;
         for (int64_t g = 0; g < steps; ++g) {
             if ((int)(g & 1) == turn) {
-                copy();
-                cp_async_wait<kAhead>();
-                __syncwarp();             // the scales were copied by other lanes
-                const unsigned char* from = smem + (ring - sbase) + out * kTurnBytes;
-                out = out == kAhead ? 0 : out + 1;
-                uint4 code[4];
+                uint2 code[4][2];         // eight codes of each 64 columns
                 float scale[4];
+                wait(codes_full(a), aph);
+                __syncwarp();
+                const unsigned char* from = smem + L::CODES + a * kCodesBytes;
+                const float* sc = reinterpret_cast<const float*>(smem + L::SCALES) + a * kStep;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    code[j] = *reinterpret_cast<const uint4*>(from + (j * 32 + lane) * 16);
-                    scale[j] = *reinterpret_cast<const float*>(from + 32 * 4 * 16 + ((lane >> 3) + 4 * j) * 4);
+                    const int r = row_of(j);
+                    const unsigned char* at = from + r * 128 + (chunk & 1) * 8;
+                    code[j][0] = *reinterpret_cast<const uint2*>(at + (((chunk >> 1) ^ (r & 7)) << 4));
+                    code[j][1] = *reinterpret_cast<const uint2*>(at + (((4 + (chunk >> 1)) ^ (r & 7)) << 4));
+                    scale[j] = sc[r];
                 }
                 wait(done(s), ph);
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = row0 + 4 * j;
-                    // 16 codes are two 16-byte chunks of the swizzled row; lanes of the
-                    // upper 64 columns store theirs the other way round, so that eight
-                    // lanes' chunks fall on eight different groups of banks
-                    const uint32_t row = x_at + (uint32_t)(s * L::STAGE + r * 128);
-                    const int flip = chunk >> 2;
-                    const uint32_t w[4] = {code[j].x, code[j].y, code[j].z, code[j].w};
+                    const int r = row_of(j);
+                    const uint32_t at = x_at + (uint32_t)(s * L::STAGE + r * 128 + ((chunk ^ (r & 7)) << 4));
+                    const uint64_t by = pack2(scale[j], scale[j]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t o[4];
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            const uint32_t two = flip ? w[2 - 2 * h + (b >> 1)] : w[2 * h + (b >> 1)];
-                            const float2 f = e4m3x2_values(two >> (16 * (b & 1)));
-                            const __nv_bfloat162 e = __floats2bfloat162_rn(f.x * scale[j], f.y * scale[j]);
+                            const uint32_t w = b < 2 ? code[j][h].x : code[j][h].y;
+                            const float2 c = e4m3x2_values(w >> (16 * (b & 1)));
+                            const float2 f = unpack2(mul2(pack2(c.x, c.y), by));
+                            const __nv_bfloat162 e = __floats2bfloat162_rn(f.x, f.y);
                             o[b] = *reinterpret_cast<const uint32_t*>(&e);
                         }
-                        const uint32_t at = row + (uint32_t)(((((chunk & 3) << 1) + (h ^ flip)) ^ (r & 7)) << 4);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o[0]), "r"(o[1]),
-                                     "r"(o[2]), "r"(o[3])
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + h * (kPlaneBytes / 2)),
+                                     "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
                                      : "memory");
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(rank == 0 ? full(s) : made(s));
+                if (lane == 0) {
+                    mbar_arrive(rank == 0 ? full(s) : made(s));
+                    mbar_arrive(codes_read(a));
+                }
+            }
+            if (++a == kAhead) {
+                a = 0;
+                aph ^= 1u;
             }
             if (++s == NS) {
                 s = 0;
@@ -453,8 +461,6 @@ int bytes_of(int type) { return type == kF32 ? 4 : 2; }
 template <int P, typename O>
 cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
     Params p;
-    p.codes = g.a.codes;
-    p.ld = g.a.ld;
     p.scales = g.a.scales;
     p.s_row = g.a.s_row;
     p.s_col = g.a.s_col;
@@ -475,8 +481,9 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * bytes_of(g.out_type)) % 32 == 0;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
-    CUtensorMap map;
-    if (!encode_rows(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, g.N, P * g.M, ld * 2, kStep))
+    CUtensorMap map, mx;
+    if (!encode_rows(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, g.N, P * g.M, ld * 2, kStep) ||
+        !encode_codes(&mx, g.a.codes, g.a.cols, g.a.rows, g.a.ld, kStep))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)Smem<P>::TOTAL + 1024;
     auto kern = fp8_wgrad_kernel<P, O>;
@@ -486,7 +493,7 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     const int tiles = p.tiles_n * p.tiles_k;
     const int pairs = sm_count() / 2;
     LaunchConfig cfg(dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), kThreads, smem, s);
-    return cudaLaunchKernelEx(&cfg.c, kern, p, map);
+    return cudaLaunchKernelEx(&cfg.c, kern, p, map, mx);
 }
 
 template <int P>

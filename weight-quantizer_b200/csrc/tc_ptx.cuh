@@ -233,6 +233,11 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
     return f;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t s) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(s));
 }
@@ -255,10 +260,10 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             : "memory");
 }
 
-// Asynchronous copy of n <= 16 bytes into 16 bytes of shared memory, the rest zeros
-// (n = 0 reads nothing).
-__device__ __forceinline__ void cp_async16_n(uint32_t dst, const void* src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// Arrives on `bar` when this thread's asynchronous copies so far are done (one of
+// the arrivals that the barrier was set up for).
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- CTA pairs -----------------------------------------------------------------
