@@ -304,61 +304,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int row0 = q * 16 + (sub >> 1) + 4 * (sub & 1);
         auto row_of = [&](int j) { return row0 + 2 * (j & 1) + 8 * (j >> 1); };
         const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes);
-        int s = 0, a = 0;
+        int s = turn, a = turn;
         uint32_t ph = 1, aph = 0;
-        const int64_t steps = (int64_t)mine * p.steps;
-        for (int64_t g = 0; g < steps; ++g) {
-            if ((int)(g & 1) == turn) {
-                uint2 code[4][2];         // eight codes of each 64 columns
-                float scale[4];
+        for (int64_t left = ((int64_t)mine * p.steps + 1 - turn) >> 1; left > 0; --left) {
+            uint2 code[4][2];         // eight codes of each 64 columns
+            float scale[4];
+            if (!try_wait_both(codes_full(a), aph, done(s), ph)) {
                 wait(codes_full(a), aph);
-                __syncwarp();
-                const unsigned char* from = smem + L::CODES + a * kCodesBytes;
-                const float* sc = reinterpret_cast<const float*>(smem + L::SCALES) + a * kStep;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = row_of(j);
-                    const unsigned char* at = from + r * 128 + (chunk & 1) * 8;
-                    code[j][0] = *reinterpret_cast<const uint2*>(at + (((chunk >> 1) ^ (r & 7)) << 4));
-                    code[j][1] = *reinterpret_cast<const uint2*>(at + (((4 + (chunk >> 1)) ^ (r & 7)) << 4));
-                    scale[j] = sc[r];
-                }
                 wait(done(s), ph);
-                __syncwarp();
+            }
+            __syncwarp();
+            const unsigned char* from = smem + L::CODES + a * kCodesBytes;
+            const float* sc = reinterpret_cast<const float*>(smem + L::SCALES) + a * kStep;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = row_of(j);
-                    const uint32_t at = x_at + (uint32_t)(s * L::STAGE + r * 128 + ((chunk ^ (r & 7)) << 4));
-                    const uint64_t by = pack2(scale[j], scale[j]);
+            for (int j = 0; j < 4; ++j) {
+                const int r = row_of(j);
+                const unsigned char* at = from + r * 128 + (chunk & 1) * 8;
+                code[j][0] = *reinterpret_cast<const uint2*>(at + (((chunk >> 1) ^ (r & 7)) << 4));
+                code[j][1] = *reinterpret_cast<const uint2*>(at + (((4 + (chunk >> 1)) ^ (r & 7)) << 4));
+                scale[j] = sc[r];
+            }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t o[4];
+            for (int j = 0; j < 4; ++j) {
+                const int r = row_of(j);
+                const uint32_t at = x_at + (uint32_t)(s * L::STAGE + r * 128 + ((chunk ^ (r & 7)) << 4));
+                const uint64_t by = pack2(scale[j], scale[j]);
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const uint32_t w = b < 2 ? code[j][h].x : code[j][h].y;
-                            const float2 c = e4m3x2_values(w >> (16 * (b & 1)));
-                            const float2 f = unpack2(mul2(pack2(c.x, c.y), by));
-                            const __nv_bfloat162 e = __floats2bfloat162_rn(f.x, f.y);
-                            o[b] = *reinterpret_cast<const uint32_t*>(&e);
-                        }
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + h * (kPlaneBytes / 2)),
-                                     "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
-                                     : "memory");
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const uint32_t w = b < 2 ? code[j][h].x : code[j][h].y;
+                        const float2 c = e4m3x2_values(w >> (16 * (b & 1)));
+                        const float2 f = unpack2(mul2(pack2(c.x, c.y), by));
+                        const __nv_bfloat162 e = __floats2bfloat162_rn(f.x, f.y);
+                        o[b] = *reinterpret_cast<const uint32_t*>(&e);
                     }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(rank == 0 ? full(s) : made(s));
-                    mbar_arrive(codes_read(a));
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + h * (kPlaneBytes / 2)),
+                                 "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                                 : "memory");
                 }
             }
-            if (++a == kAhead) {
-                a = 0;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(rank == 0 ? full(s) : made(s));
+                mbar_arrive(codes_read(a));
+            }
+            a += 2;
+            if (a >= kAhead) {
+                a -= kAhead;
                 aph ^= 1u;
             }
-            if (++s == NS) {
-                s = 0;
+            s += 2;
+            if (s >= NS) {
+                s -= NS;
                 ph ^= 1u;
             }
         }

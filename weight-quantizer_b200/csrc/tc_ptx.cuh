@@ -76,6 +76,20 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// One probe of two barriers' phases at once (their latencies overlap).
+__device__ __forceinline__ bool try_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+        "and.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+        : "memory");
+    return ok != 0;
+}
+
 // Arrives on `bar` when the MMAs issued so far are done; in a CTA pair on the
 // barrier at the same offset of both CTAs.
 template <int CTAS>
