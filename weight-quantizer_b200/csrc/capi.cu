@@ -585,7 +585,8 @@ int wq_fp8_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64
     if (block_rows != 1 && ((rows + 127) / 128) * ((cols + 127) / 128) > kMaxDim) return WQ_E_TOO_LARGE;
     if (rows == 0 || cols == 0) return WQ_OK;
     if (x == nullptr || codes == nullptr || scales == nullptr) return WQ_E_NULL;
-    const wq::Fp8Quantize q{x, x_type, rows, cols, ldx, codes, ld, scales, s_row, s_col, block_rows};
+    const wq::Fp8Quantize q{x,      x_type, rows,  cols,       ldx,     codes, ld,
+                            scales, s_row,  s_col, block_rows, nullptr, 0};
     cudaError_t e = wq::launch_fp8_quantize(q, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
@@ -643,7 +644,7 @@ int wq_fp8_gemm(const uint8_t* a, int64_t M, int64_t K, int64_t lda, const float
     const wq::Fp8Operand ao{a, M, K, lda, a_scales, as_row, as_col, 1};
     const wq::Fp8Operand wo{w, w_rows, w_cols, ldw, w_scales, ws_row, ws_col, wq::kFp8Block};
     const wq::Fp8Gemm g{ao, wo, transpose ? 1 : 0, M, N, K, bias, bias_type, out, out_type, ldo};
-    cudaError_t e = wq::launch_fp8_gemm(g, workspace, static_cast<cudaStream_t>(stream));
+    cudaError_t e = wq::launch_fp8_gemm(g, workspace, false, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
 
@@ -684,11 +685,12 @@ int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_t ldx, 
     const wq::Fp8Operand wo{w, w_rows, w_cols, ldw, w_scales, ws_row, ws_col, wq::kFp8Block};
     const wq::Fp8Gemm g{ao, wo, transpose ? 1 : 0, M, N, K, bias, bias_type, out, out_type, ldo};
     if (K > 0) {
-        const wq::Fp8Quantize q{x, x_type, M, K, ldx, codes, ld, scales, 1, M, 1};
+        const wq::Fp8Quantize q{x, x_type, M, K, ldx, codes, ld, scales, 1, M, 1, static_cast<unsigned int*>(rest),
+                                (int64_t)(wq::fp8_gemm_zeroed_bytes(M, N, K) / 4)};
         cudaError_t e = wq::launch_fp8_quantize(q, s);
         if (e != cudaSuccess) return cuda_fail(e);
     }
-    cudaError_t e = wq::launch_fp8_gemm(g, rest, s);
+    cudaError_t e = wq::launch_fp8_gemm(g, rest, true, s);
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
 

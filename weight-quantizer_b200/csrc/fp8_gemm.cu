@@ -297,6 +297,323 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (warp == 1) tmem_free<2>(tmem, 512);
 }
 
+// ---- few rows: weights stream by, the work split evenly ------------------------------
+//
+// With few rows of a the bound is the weights' bytes (and, once they are in L2, the
+// latency of each block). One CTA per SM; the MMA's rows (tensor-memory lanes) are
+// 128 rows of w, its columns `bn` <= BN rows of a. The work is cut into units of 128
+// rows of w x one block, and every CTA takes an equal run of them, wherever tiles
+// begin or end (224 row tiles on 148 SMs would leave a quarter of them idle in the
+// second round). A CTA that holds a whole tile writes y; the others put their sums
+// into the workspace, and the last to arrive at a tile adds them in CTA order (a
+// fixed order, whoever is last) and writes y.
+//
+// Warp 0 loads units (TMA) into a ring that spans ten of them (180 KB in flight per
+// SM); warps 1 and 2 issue the MMAs of even and odd units; warp 3 copies the unit's
+// scales (asynchronous 4-byte copies); the other warps add each unit's sums, times
+// the scales, to registers. Up to eight units' sums are in tensor memory, so no
+// hand-off waits for another.
+
+template <int BN>
+struct Few {
+    static constexpr int SUM_WARPS = BN > 64 ? 8 : 4;
+    static constexpr int COLS = BN > 64 ? BN / 2 : BN;          // columns per summing warp
+    static constexpr int THREADS = 128 + 32 * SUM_WARPS;
+    static constexpr int BUFS = BN > 64 ? 4 : 8;                // even: each issuing warp has its own
+    static constexpr uint32_t TMEM = BUFS * BN;
+    static constexpr int STAGE = kOperandBytes + BN * 128;
+    static constexpr int STAGES = (BN > 64 ? 192 : 200) * 1024 / STAGE / 2 * 2;   // even likewise
+    static constexpr int SCALES = STAGES * STAGE;               // per buffer BN of a, one of w
+    static constexpr int SCALE_BYTES = (BN + 4) * 4;
+    static constexpr int BAR = SCALES + BUFS * SCALE_BYTES;
+    // full, done per stage; scales there, sums empty per buffer
+    static constexpr int TMEM_SLOT = BAR + 8 * (2 * STAGES + 2 * BUFS);
+    static constexpr int FLAG = TMEM_SLOT + 8;
+    static constexpr int TOTAL = TMEM_SLOT + 16;
+    static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
+};
+
+struct FewParams {
+    const float* sa;
+    int64_t sa_row, sa_col;
+    const float* sw;
+    int64_t sw_n, sw_k;
+    const void* bias;
+    int bias_type;
+    void* out;
+    int out_type;
+    int64_t ldo;
+    int M, N, blocks;
+    int tiles_a, bn;         // tiles of bn rows of a
+    int64_t units;
+    float* part;             // two slots of 128 x BN sums per CTA
+    unsigned int* arrived;   // per tile, zeroed before the launch
+    bool weights_ready;      // w was complete before the previous kernel let this one start
+    unsigned int* fault;
+};
+
+__device__ __forceinline__ int64_t first_unit(int64_t cta, int64_t units, int64_t ctas) { return cta * units / ctas; }
+__device__ __forceinline__ int64_t cta_of(int64_t unit, int64_t units, int64_t ctas) {
+    return ((unit + 1) * ctas - 1) / units;
+}
+
+template <int BN, bool WT>
+__global__ void __launch_bounds__(Few<BN>::THREADS, 1)
+    fp8_gemm_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap map_a,
+                        const __grid_constant__ CUtensorMap map_w) {
+    using L = Few<BN>;
+    constexpr int NS = L::STAGES, NB = L::BUFS;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_addr(smem);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
+    auto bar = [&](int i) -> uint32_t { return sbase + L::BAR + 8u * (uint32_t)i; };
+    auto full = [&](int s) { return bar(s); };
+    auto done = [&](int s) { return bar(NS + s); };
+    auto scaled = [&](int b) { return bar(2 * NS + b); };
+    auto sums_empty = [&](int b) { return bar(2 * NS + NB + b); };
+    launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(done(s), 1);
+        }
+        for (int b = 0; b < NB; ++b) {
+            mbar_init(scaled(b), 32);
+            mbar_init(sums_empty(b), L::SUM_WARPS);
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 1) tmem_alloc<1>(sbase + L::TMEM_SLOT, L::TMEM);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (!p.weights_ready || warp != 0) grid_wait();   // nothing above reads global memory
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_SLOT);
+    const int64_t u0 = first_unit(blockIdx.x, p.units, gridDim.x), u1 = first_unit(blockIdx.x + 1, p.units, gridDim.x);
+    bool faulted = false;
+    auto wait = [&](uint32_t b, uint32_t parity) {
+        if (!faulted && !mbar_wait_bounded(b, parity)) {
+            faulted = true;
+            atomicOr(p.fault, 1u);
+        }
+    };
+
+    if (warp == 0) {
+        const uint32_t bytes = (uint32_t)(kOperandBytes + p.bn * 128);
+        int tile = (int)(u0 / p.blocks), b = (int)(u0 - (int64_t)tile * p.blocks);
+        auto load_w = [&](int s, int tile, int b) {
+            const int r0 = tile / p.tiles_a * 128;
+            mbar_arrive_expect_tx(full(s), bytes);
+            if constexpr (WT) tma_box<1>(sbase + (uint32_t)(s * L::STAGE), &map_w, r0, b * 128, full(s));
+            else tma_box<1>(sbase + (uint32_t)(s * L::STAGE), &map_w, b * 128, r0, full(s));
+        };
+        auto load_a = [&](int s, int tile, int b) {
+            tma_box<1>(sbase + (uint32_t)(s * L::STAGE + kOperandBytes), &map_a, b * 128, tile % p.tiles_a * p.bn, full(s));
+        };
+        // the first round's weights may come before the previous kernel (which makes
+        // a's codes) is over
+        const int ahead = (int)min((int64_t)NS, u1 - u0);
+        {
+            int t = tile, c = b;
+            for (int s = 0; s < ahead; ++s) {
+                if (elect_one()) load_w(s, t, c);
+                __syncwarp();
+                if (++c == p.blocks) c = 0, ++t;
+            }
+        }
+        if (p.weights_ready) grid_wait();
+        int s = 0;
+        uint32_t ph = 1;
+        for (int64_t u = u0; u < u1; ++u) {
+            const bool loaded = u - u0 < ahead;
+            if (!loaded) wait(done(s), ph);
+            __syncwarp();
+            if (elect_one()) {
+                if (!loaded) load_w(s, tile, b);
+                load_a(s, tile, b);
+            }
+            __syncwarp();
+            if (++b == p.blocks) b = 0, ++tile;
+            if (++s == NS) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+        // every copy this warp started has been read before the CTA goes
+        // (a stage that was never filled passes at once)
+        for (int i = 0; i < NS; ++i) {
+            if (!mbar_wait_bounded(done(s), ph)) atomicOr(p.fault, 1u);
+            if (++s == NS) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+    } else if (warp < 3) {
+        const uint32_t idesc = mma_idesc(0, WT, false, 128, p.bn);
+        const uint64_t desc0 = sw128_matrix(sbase);
+        int s = warp - 1, buf = warp - 1;
+        uint32_t ph = 0, bph = 1;
+        for (int64_t u = u0 + warp - 1; u < u1; u += 2) {
+            if (!try_wait_both(full(s), ph, sums_empty(buf), bph)) {
+                wait(full(s), ph);
+                wait(sums_empty(buf), bph);
+            }
+            __syncwarp();
+            tc_after();
+            if (elect_one()) {
+                const uint64_t dw = desc0 + (uint64_t)(s * (L::STAGE >> 4));
+                const uint64_t da = dw + (uint64_t)(kOperandBytes >> 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)   // 32 codes: 32 bytes of a row, or 32 rows of 128 bytes
+                    mma_f8<1>(tmem + (uint32_t)(buf * BN), dw + (WT ? 256u : 2u) * k, da + 2u * k, idesc, k > 0);
+                mma_done<1>(done(s));
+            }
+            __syncwarp();
+            s += 2;
+            if (s >= NS) {
+                s -= NS;
+                ph ^= 1u;
+            }
+            buf += 2;
+            if (buf >= NB) {
+                buf -= NB;
+                bph ^= 1u;
+            }
+        }
+    } else if (warp == 3) {
+        // scales of the unit's block: a's rows of the tile (beyond the last: 0), and w's
+        int tile = (int)(u0 / p.blocks), b = (int)(u0 - (int64_t)tile * p.blocks);
+        int buf = 0;
+        uint32_t bph = 1;
+        for (int64_t u = u0; u < u1; ++u) {
+            wait(sums_empty(buf), bph);
+            __syncwarp();
+            const int m0 = tile % p.tiles_a * p.bn;
+            const uint32_t to = sbase + (uint32_t)(L::SCALES + buf * L::SCALE_BYTES);
+#pragma unroll
+            for (int i = 0; i < (BN + 31) / 32; ++i) {
+                const int c = i * 32 + lane;
+                const bool some = c < p.bn && m0 + c < p.M;
+                if (c < BN) cp_async4_s(to + c * 4, some ? p.sa + (m0 + c) * p.sa_row + b * p.sa_col : p.sa, some);
+            }
+            if (lane == 0) cp_async4_s(to + BN * 4, p.sw + tile / p.tiles_a * p.sw_n + b * p.sw_k, true);
+            cp_async_arrive(scaled(buf));
+            if (++b == p.blocks) b = 0, ++tile;
+            if (++buf == NB) {
+                buf = 0;
+                bph ^= 1u;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const int row = q * 32 + lane;
+        constexpr int C = L::COLS;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * C);
+        int s = 0, buf = 0;
+        uint32_t ph = 0, bph = 0;
+        int64_t u = u0;
+        while (u < u1) {
+            // the part of a tile that this CTA holds
+            const int tile = (int)(u / p.blocks);
+            const int64_t t0 = (int64_t)tile * p.blocks, t1 = t0 + p.blocks;
+            const int64_t from = u, to = min(u1, t1);
+            uint64_t acc[C / 2];
+#pragma unroll
+            for (int c = 0; c < C / 2; ++c) acc[c] = 0;
+            for (; u < to; ++u) {
+                if (!try_wait_both(done(s), ph, scaled(buf), bph)) {
+                    wait(done(s), ph);
+                    wait(scaled(buf), bph);
+                }
+                __syncwarp();
+                tc_after();
+                const float* sc = reinterpret_cast<const float*>(smem + L::SCALES + buf * L::SCALE_BYTES);
+                const float w = sc[BN];
+                const uint64_t w2 = pack2(w, w);
+#pragma unroll
+                for (int c0 = 0; c0 < C; c0 += (C < 32 ? C : 32)) {
+                    constexpr int STEP = C < 32 ? C : 32;
+                    uint64_t v[STEP / 2];
+                    tmem_pairs(taddr + (uint32_t)(buf * BN + c0), v);
+#pragma unroll
+                    for (int c = 0; c < STEP / 4; ++c) {
+                        const float4 f = *reinterpret_cast<const float4*>(sc + half * C + c0 + 4 * c);
+                        fma2(acc[c0 / 2 + 2 * c], v[2 * c], mul2(pack2(f.x, f.y), w2));
+                        fma2(acc[c0 / 2 + 2 * c + 1], v[2 * c + 1], mul2(pack2(f.z, f.w), w2));
+                    }
+                }
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sums_empty(buf));
+                if (++s == NS) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+                if (++buf == NB) {
+                    buf = 0;
+                    bph ^= 1u;
+                }
+            }
+            float y[C];
+#pragma unroll
+            for (int c = 0; c < C / 2; ++c) {
+                const float2 f = unpack2(acc[c]);
+                y[2 * c] = f.x;
+                y[2 * c + 1] = f.y;
+            }
+            bool write = true;
+            if (from != t0 || to != t1) {
+                const int64_t ctas = gridDim.x;
+                float* mine = p.part + (2 * (int64_t)blockIdx.x + (from == u0 ? 0 : 1)) * (128 * BN);
+#pragma unroll
+                for (int c = 0; c < C; ++c) mine[(half * C + c) * 128 + row] = y[c];
+                __threadfence();
+                named_barrier(1, 32 * L::SUM_WARPS);
+                volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
+                const int64_t c0 = cta_of(t0, p.units, ctas), c1 = cta_of(t1 - 1, p.units, ctas);
+                if (warp == 4 && lane == 0) *flag = atomicAdd(p.arrived + tile, 1u) == (unsigned)(c1 - c0);
+                named_barrier(1, 32 * L::SUM_WARPS);
+                write = *flag != 0u;
+                named_barrier(1, 32 * L::SUM_WARPS);   // the flag has been read
+                if (write) {
+                    __threadfence();
+#pragma unroll
+                    for (int c = 0; c < C; ++c) y[c] = 0.0f;
+                    for (int64_t cta = c0; cta <= c1; ++cta) {
+                        const int64_t b = first_unit(cta, p.units, ctas);
+                        const float* src = p.part + (2 * cta + (b >= t0 ? 0 : 1)) * (128 * BN);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) y[c] += __ldcg(src + (half * C + c) * 128 + row);
+                    }
+                }
+            }
+            const int n = tile / p.tiles_a * 128 + row;
+            if (write && n < p.N) {
+                const float bias = load_any(p.bias, p.bias_type, n);
+                const int m0 = tile % p.tiles_a * p.bn + half * C;
+                const int cols = min(C, min(p.bn - half * C, p.M - m0));
+                const int64_t at = m0 * p.ldo + n;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    if (c < cols) {
+                        const float v = y[c] + bias;
+                        if (p.out_type == kBf16) static_cast<__nv_bfloat16*>(p.out)[at + c * p.ldo] = from_f32<__nv_bfloat16>(v);
+                        else if (p.out_type == kF16) static_cast<__half*>(p.out)[at + c * p.ldo] = from_f32<__half>(v);
+                        else static_cast<float*>(p.out)[at + c * p.ldo] = v;
+                    }
+                }
+            }
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 1) tmem_free<1>(tmem, L::TMEM);
+}
+
 // ---- host side ------------------------------------------------------------------------
 
 int type_bytes(int t) { return t == kF32 ? 4 : 2; }
@@ -351,11 +668,94 @@ cudaError_t launch_pair(const Fp8Gemm& g, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
 }
 
+// ---- few rows: plan ----
+
+// Tiles of a's rows: as few as hold at most 128 each, of equal size in steps of 16.
+int few_tiles(int64_t M) { return (int)((M + 127) / 128); }
+int few_bn(int64_t M) {
+    const int64_t t = few_tiles(M);
+    return (int)(((M + t - 1) / t + 15) / 16 * 16);
+}
+int few_width(int64_t M) {
+    const int bn = few_bn(M);
+    return bn <= 16 ? 16 : (bn <= 32 ? 32 : (bn <= 64 ? 64 : 128));
+}
+int64_t few_row_tiles(int64_t N) { return (N + 127) / 128; }
+int64_t few_ctas(int64_t M, int64_t N, int64_t K) {
+    const int64_t units = few_row_tiles(N) * few_tiles(M) * ((K + 127) / 128);
+    return units < sm_count() ? units : sm_count();
+}
+size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
+size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
+    return round_up((size_t)few_ctas(M, N, K) * 2 * 128 * (size_t)few_width(M) * 4);
+}
+size_t few_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)few_row_tiles(N) * few_tiles(M) * 4); }
+
+bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= 128; }
+
+template <int BN, bool WT>
+cudaError_t launch_few_t(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
+    CUtensorMap ma, mw;
+    if (!encode_codes(&ma, g.a.codes, g.a.cols, g.a.rows, g.a.ld, (uint32_t)p.bn) ||
+        !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, 128))
+        return cudaErrorInvalidValue;
+    const size_t smem = (size_t)Few<BN>::TOTAL + 1024;
+    auto kern = fp8_gemm_few_kernel<BN, WT>;
+    static std::atomic<int> ready[kMaxDevices];
+    cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, 0, ready);
+    if (e != cudaSuccess) return e;
+    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K)), Few<BN>::THREADS, smem, s);
+    return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
+}
+
+template <bool WT>
+cudaError_t launch_few(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
+    FewParams p;
+    p.sa = g.a.scales;
+    p.sa_row = g.a.s_row;
+    p.sa_col = g.a.s_col;
+    p.sw = g.w.scales;
+    p.sw_n = WT ? g.w.s_col : g.w.s_row;
+    p.sw_k = WT ? g.w.s_row : g.w.s_col;
+    p.bias = g.bias;
+    p.bias_type = g.bias_type;
+    p.out = g.out;
+    p.out_type = g.out_type;
+    p.ldo = g.ldo;
+    p.M = (int)g.M;
+    p.N = (int)g.N;
+    p.blocks = (int)((g.K + 127) / 128);
+    p.tiles_a = few_tiles(g.M);
+    p.bn = few_bn(g.M);
+    p.units = few_row_tiles(g.N) * p.tiles_a * p.blocks;
+    p.arrived = static_cast<unsigned int*>(workspace);
+    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + few_arrived_bytes(g.M, g.N));
+    p.weights_ready = prepared;
+    p.fault = fault_word();
+    if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
+    if (!prepared) {
+        cudaError_t e = cudaMemsetAsync(workspace, 0, few_arrived_bytes(g.M, g.N), s);
+        if (e != cudaSuccess) return e;
+    }
+    switch (few_width(g.M)) {
+        case 16: return launch_few_t<16, WT>(g, p, s);
+        case 32: return launch_few_t<32, WT>(g, p, s);
+        case 64: return launch_few_t<64, WT>(g, p, s);
+        default: return launch_few_t<128, WT>(g, p, s);
+    }
+}
+
 }  // namespace
 
-size_t fp8_gemm_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return few_rows(M, N, K) ? few_arrived_bytes(M, N) + few_part_bytes(M, N, K) : 0;
+}
 
-cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void*, cudaStream_t s) {
+size_t fp8_gemm_zeroed_bytes(int64_t M, int64_t N, int64_t K) {
+    return few_rows(M, N, K) ? few_arrived_bytes(M, N) : 0;
+}
+
+cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
     if (g.K == 0) {
         const int64_t n = (g.M * g.N + 255) / 256;
         const unsigned grid = (unsigned)(n < 65536 ? n : 65536);
@@ -368,6 +768,8 @@ cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void*, cudaStream_t s) {
             fill_rows_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(g.out), g.M, g.N, g.ldo, g.bias, g.bias_type);
         return cudaGetLastError();
     }
+    if (few_rows(g.M, g.N, g.K))
+        return g.transpose ? launch_few<true>(g, workspace, prepared, s) : launch_few<false>(g, workspace, prepared, s);
     return g.transpose ? launch_pair<true>(g, s) : launch_pair<false>(g, s);
 }
 

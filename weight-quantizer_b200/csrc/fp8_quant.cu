@@ -15,6 +15,8 @@
 // or 4/16384 (tiles) for the scale.
 #include "fp8_types.cuh"
 #include "kernels.h"
+#include "launch.h"
+#include "tc_ptx.cuh"
 
 namespace wq {
 namespace {
@@ -62,7 +64,13 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                        int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc,
                                                        bool vec_out, float* __restrict__ scales, int64_t s_row,
-                                                       int64_t s_col) {
+                                                       int64_t s_col, unsigned int* zero, int64_t zeros) {
+    // what follows may start once every CTA is past the work before this launch
+    grid_wait();
+    launch_dependents();
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < zeros;
+         i += (int64_t)gridDim.x * gridDim.y * 256)
+        zero[i] = 0;
     const int64_t row = (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 4);
     const int sub = threadIdx.x & 15;
     const int64_t nb = (cols + kFp8Block - 1) / kFp8Block;
@@ -186,12 +194,9 @@ cudaError_t quantize_t(const Fp8Quantize& q, cudaStream_t s) {
     if (q.block_rows == 1) {
         const dim3 grid((unsigned)((q.rows + kRowsPerCta - 1) / kRowsPerCta),
                         (unsigned)((nb + kBlocksPerThread - 1) / kBlocksPerThread));
-        if (vec)
-            fp8_rows_kernel<T, true><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out, q.scales,
-                                                          q.s_row, q.s_col);
-        else
-            fp8_rows_kernel<T, false><<<grid, 256, 0, s>>>(x, q.rows, q.cols, q.ldx, q.codes, q.ldc, vec_out, q.scales,
-                                                           q.s_row, q.s_col);
+        LaunchConfig cfg(grid, 256, 0, s);
+        return cudaLaunchKernelEx(&cfg.c, vec ? fp8_rows_kernel<T, true> : fp8_rows_kernel<T, false>, x, q.rows, q.cols,
+                                  q.ldx, q.codes, q.ldc, vec_out, q.scales, q.s_row, q.s_col, q.zero, q.zeros);
     } else {
         const unsigned grid = (unsigned)((q.rows + kFp8Block - 1) / kFp8Block * nb);
         if (vec)

@@ -152,6 +152,8 @@ struct Fp8Quantize {
     float* scales;
     int64_t s_row, s_col;
     int block_rows;
+    unsigned int* zero;   // words to set to 0 on the way, or nullptr
+    int64_t zeros;
 };
 cudaError_t launch_fp8_quantize(const Fp8Quantize& q, cudaStream_t s);
 cudaError_t launch_fp8_values(const Fp8Operand& a, void* out, int out_type, int64_t ldo, cudaStream_t s);
@@ -172,7 +174,11 @@ struct Fp8Gemm {
     int64_t ldo;
 };
 size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
-cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, cudaStream_t s);
+// `prepared`: the previous launch on the stream is launch_fp8_quantize, which has
+// zeroed the first fp8_gemm_zeroed_bytes() of the workspace and waited for all work
+// before it.
+size_t fp8_gemm_zeroed_bytes(int64_t M, int64_t N, int64_t K);
+cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s);
 
 // dw[n, k] (+)= sum_m dy[m, n] x^[m, k], x^ the values of a with one scale per
 // row and block.
