@@ -680,6 +680,9 @@ def chol_inverse_upper(a: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 # ---- blocks of 8-bit floating point -------------------------------------------
+#
+# A small layer's kernels take a few microseconds, so the host's part of a call
+# counts: no helper objects, one allocation per result, one C call.
 
 FP8_BLOCK = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # wq_dtype
@@ -692,96 +695,101 @@ def _dtype(t: torch.dtype, what: str) -> int:
     return code
 
 
-class _on:
-    """Makes a tensor's device the current one for a launch (nothing to do when it already is)."""
-
-    __slots__ = ("index", "prev")
-
-    def __init__(self, device: torch.device) -> None:
-        self.index = device.index
-
-    def __enter__(self) -> None:
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc: object) -> None:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+def _fp8_device(first: torch.Tensor, *others: torch.Tensor) -> torch.device:
+    if not first.is_cuda:
+        raise ValueError("dequant kernel inputs must be CUDA tensors")
+    dev = first.device
+    for t in others:
+        if t.device != dev:
+            _cuda_device([first, *others])
+    return dev
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x [rows, cols] with unit column stride and rows that do not overlap (a copy where x has neither)."""
-    if x.stride(1) == 1 and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1):
-        return x
-    return x if x.shape[1] == 1 and x.stride(0) >= 1 else x.contiguous()
+def _fp8_call(fn: Any, dev: torch.device, args: tuple[Any, ...], check_faults: bool = False) -> None:
+    """One entry point on the device's current stream, with that device current for the launch."""
+    prev = torch.cuda.current_device()
+    if prev == dev.index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(prev))
+    else:
+        torch.cuda.set_device(dev)
+        try:
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        finally:
+            torch.cuda.set_device(prev)
+    if status != WQ_OK:
+        _check(status)
+    if check_faults and _fault_check and not torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device(dev):
+            _raise_on_fault()
 
 
-def _ld(x: torch.Tensor) -> int:
-    return int(x.stride(0)) if x.shape[0] > 1 else max(int(x.shape[1]), 1)
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x [rows, cols] with unit column stride and rows that do not overlap (a copy where x has neither), and its
+    row stride."""
+    rows, cols = x.shape
+    s0, s1 = x.stride()
+    if s1 == 1 or cols == 1:
+        if rows <= 1:
+            return x, max(cols, 1)
+        if s0 >= max(cols, 1):
+            return x, s0
+    x = x.contiguous()
+    return x, max(cols, 1)
 
 
 def _codes_arg(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Codes as the products read them (16-byte aligned, rows a multiple of 16 bytes apart) and their row stride:
     codes laid out otherwise are copied."""
     rows, cols = codes.shape
-    if codes.numel() == 0:
-        return codes, (cols + 15) // 16 * 16
-    if codes.data_ptr() % 16 == 0 and (codes.stride(1) == 1 or cols == 1):
-        if rows == 1:
-            return codes, (cols + 15) // 16 * 16
-        if codes.stride(0) % 16 == 0 and codes.stride(0) >= cols:
-            return codes, int(codes.stride(0))
     pitch = (cols + 15) // 16 * 16
+    s0, s1 = codes.stride()
+    if codes.numel() == 0:
+        return codes, pitch
+    if s1 == 1 or cols == 1:
+        if codes.data_ptr() % 16 == 0:
+            if rows == 1:
+                return codes, pitch
+            if s0 % 16 == 0 and s0 >= cols:
+                return codes, s0
+        plain = codes.view(torch.uint8)
+    else:
+        plain = codes.contiguous().view(torch.uint8)
     kept = torch.empty((rows, pitch), dtype=torch.uint8, device=codes.device)
-    kept[:, :cols].copy_(codes.view(torch.uint8) if codes.stride(1) == 1 or cols == 1
-                         else codes.contiguous().view(torch.uint8))
+    kept[:, :cols].copy_(plain)
     return kept, pitch
-
-
-def _workspace(n: int, dev: torch.device) -> torch.Tensor | None:
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
-
-
-def _after_fp8(status: int) -> None:
-    if status != WQ_OK:
-        _check(status)
-    if _fault_check and not torch.cuda.is_current_stream_capturing():
-        _raise_on_fault()
 
 
 def fp8_quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of x [rows, cols]; codes are a view of rows padded to 16 bytes."""
     x_type = _dtype(x.dtype, "x")
-    dev = _cuda_device([x])
-    x = _rows(x)
+    dev = _fp8_device(x)
+    x, ldx = _rows(x)
     rows, cols = x.shape
     pitch = (cols + 15) // 16 * 16
     nb = (cols + FP8_BLOCK - 1) // FP8_BLOCK
     codes = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=dev)
     if block_rows == 1:
-        scales = torch.empty((nb, rows), dtype=torch.float32, device=dev).t()
+        s_row, s_col = 1, max(rows, 1)   # one block's scales of all rows side by side
+        scales = torch.empty_strided((rows, nb), (1, s_col), dtype=torch.float32, device=dev)
     else:
+        s_row, s_col = max(nb, 1), 1
         scales = torch.empty(((rows + FP8_BLOCK - 1) // FP8_BLOCK, nb), dtype=torch.float32, device=dev)
-    with _on(dev):
-        status = library().wq_fp8_quantize(
-            x.data_ptr(), x_type, rows, cols, _ld(x), block_rows, codes.data_ptr(), pitch, scales.data_ptr(),
-            scales.stride(0), scales.stride(1), _stream(dev))
-    _check(status)
+    _fp8_call(library().wq_fp8_quantize, dev,
+              (x.data_ptr(), x_type, rows, cols, ldx, block_rows, codes.data_ptr(), pitch, scales.data_ptr(), s_row,
+               s_col))
     return (codes if pitch == cols else codes[:, :cols]), scales
 
 
 def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, block_rows: int, dtype: torch.dtype) -> torch.Tensor:
     """code * scale as a dense [rows, cols] tensor of ``dtype``."""
     out_type = _dtype(dtype, "dtype")
-    dev = _cuda_device([codes, scales])
-    codes = _rows(codes)
+    dev = _fp8_device(codes, scales)
+    codes, ld = _rows(codes)
     rows, cols = codes.shape
     out = torch.empty((rows, cols), dtype=dtype, device=dev)
-    with _on(dev):
-        _check(library().wq_fp8_dequantize(
-            codes.data_ptr(), rows, cols, _ld(codes), block_rows, scales.data_ptr(), scales.stride(0),
-            scales.stride(1), out.data_ptr(), out_type, max(cols, 1), _stream(dev)))
+    _fp8_call(library().wq_fp8_dequantize, dev,
+              (codes.data_ptr(), rows, cols, ld, block_rows, scales.data_ptr(), *scales.stride(), out.data_ptr(),
+               out_type, max(cols, 1)))
     return out
 
 
@@ -793,7 +801,7 @@ def _out_arg(out: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype,
         raise ValueError(f"out must be a {dtype} [{rows}, {cols}] tensor on the inputs' device")
     if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
         raise ValueError("out must have unit column stride and rows that do not overlap")
-    return out, (int(out.stride(0)) if rows > 1 else max(cols, 1))
+    return out, (out.stride(0) if rows > 1 else max(cols, 1))
 
 
 def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor,
@@ -802,42 +810,40 @@ def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor | None, w: torch.Tensor, w_
     """a w^T (+ bias), or a w with ``transpose``: a [M, K] codes with their scales, or (``a_scales`` None) a 16- or
     32-bit matrix that the call quantizes."""
     out_type = _dtype(out_dtype, "out_dtype")
-    dev = _cuda_device([a, w, w_scales] + ([] if a_scales is None else [a_scales]))
+    dev = _fp8_device(a, w, w_scales) if a_scales is None else _fp8_device(a, a_scales, w, w_scales)
     M, K = a.shape
     w_rows, w_cols = w.shape
-    N = w_cols if transpose else w_rows
-    if (w_rows if transpose else w_cols) != K:
-        raise ValueError(f"a has trailing dim {K}, weight expects {w_rows if transpose else w_cols}")
-    bias_type = 0
+    N, inner = (w_cols, w_rows) if transpose else (w_rows, w_cols)
+    if inner != K:
+        raise ValueError(f"a has trailing dim {K}, weight expects {inner}")
+    bias_ptr, bias_type = None, 0
     if bias is not None:
         bias_type = _dtype(bias.dtype, "bias")
         if bias.device != dev:
             raise ValueError("bias must be on the inputs' device")
-        bias = bias.reshape(-1).contiguous()
         if bias.numel() != N:
             raise ValueError("bias does not match the output's columns")
+        bias = bias.reshape(-1).contiguous()
+        bias_ptr = bias.data_ptr()
     y, ldo = _out_arg(out, M, N, out_dtype, dev)
     w, ldw = _codes_arg(w)
     lib = library()
-    with _on(dev):
-        if a_scales is None:
-            x_type = _dtype(a.dtype, "a")
-            a = _rows(a)
-            nws = lib.wq_fp8_linear_workspace_bytes(M, N, K)
-            ws = _workspace(nws, dev)
-            status = lib.wq_fp8_linear(
-                a.data_ptr(), x_type, M, K, _ld(a), w.data_ptr(), w_rows, w_cols, ldw, w_scales.data_ptr(),
-                w_scales.stride(0), w_scales.stride(1), int(transpose), _ptr(bias), bias_type, y.data_ptr(), out_type,
-                ldo, _ptr(ws), nws, _stream(dev))
-        else:
-            a, lda = _codes_arg(a)
-            nws = lib.wq_fp8_gemm_workspace_bytes(M, N, K)
-            ws = _workspace(nws, dev)
-            status = lib.wq_fp8_gemm(
-                a.data_ptr(), M, K, lda, a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), w.data_ptr(),
-                w_rows, w_cols, ldw, w_scales.data_ptr(), w_scales.stride(0), w_scales.stride(1), int(transpose),
-                _ptr(bias), bias_type, y.data_ptr(), out_type, ldo, _ptr(ws), nws, _stream(dev))
-        _after_fp8(status)
+    weight = (w.data_ptr(), w_rows, w_cols, ldw, w_scales.data_ptr(), *w_scales.stride(), int(transpose), bias_ptr,
+              bias_type, y.data_ptr(), out_type, ldo)
+    ws: torch.Tensor | None = None
+    ws_ptr = None
+    nws = (lib.wq_fp8_linear_workspace_bytes if a_scales is None else lib.wq_fp8_gemm_workspace_bytes)(M, N, K)
+    if nws:
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        ws_ptr = ws.data_ptr()
+    if a_scales is None:
+        x_type = _dtype(a.dtype, "a")
+        a, ldx = _rows(a)
+        _fp8_call(lib.wq_fp8_linear, dev, (a.data_ptr(), x_type, M, K, ldx, *weight, ws_ptr, nws), True)
+    else:
+        a, lda = _codes_arg(a)
+        _fp8_call(lib.wq_fp8_gemm, dev, (a.data_ptr(), M, K, lda, a_scales.data_ptr(), *a_scales.stride(), *weight,
+                                         ws_ptr, nws), True)
     return y
 
 
@@ -846,22 +852,20 @@ def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     """dw [N, K] = dy^T (code * scale), added to ``out`` with ``accumulate``."""
     dy_type = _dtype(dy.dtype, "dy")
     out_type = _dtype(out_dtype, "out_dtype")
-    dev = _cuda_device([dy, codes, scales])
+    dev = _fp8_device(dy, codes, scales)
     M, N = dy.shape
     if codes.shape[0] != M:
         raise ValueError(f"dy has {M} rows, the checkpoint {codes.shape[0]}")
     K = codes.shape[1]
     dw, ldw = _out_arg(out, N, K, out_dtype, dev)
-    dy = _rows(dy)
+    dy, ldy = _rows(dy)
     codes, ld = _codes_arg(codes)
     lib = library()
     nws = lib.wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type)
-    with _on(dev):
-        ws = _workspace(nws, dev)
-        status = lib.wq_fp8_weight_grad(
-            dy.data_ptr(), dy_type, M, N, _ld(dy), codes.data_ptr(), K, ld, scales.data_ptr(), scales.stride(0),
-            scales.stride(1), dw.data_ptr(), out_type, ldw, int(accumulate), _ptr(ws), nws, _stream(dev))
-        _after_fp8(status)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _fp8_call(lib.wq_fp8_weight_grad, dev,
+              (dy.data_ptr(), dy_type, M, N, ldy, codes.data_ptr(), K, ld, scales.data_ptr(), *scales.stride(),
+               dw.data_ptr(), out_type, ldw, int(accumulate), None if ws is None else ws.data_ptr(), nws), True)
     return dw
 
 
@@ -869,11 +873,9 @@ def column_sum(x: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
     """The sum of x [rows, cols] over its rows, in fp32, rounded once to ``out_dtype``."""
     x_type = _dtype(x.dtype, "x")
     out_type = _dtype(out_dtype, "out_dtype")
-    dev = _cuda_device([x])
-    x = _rows(x)
+    dev = _fp8_device(x)
+    x, ldx = _rows(x)
     rows, cols = x.shape
     out = torch.empty(cols, dtype=out_dtype, device=dev)
-    with _on(dev):
-        _check(library().wq_column_sum(x.data_ptr(), x_type, rows, cols, _ld(x), out.data_ptr(), out_type,
-                                       _stream(dev)))
+    _fp8_call(library().wq_column_sum, dev, (x.data_ptr(), x_type, rows, cols, ldx, out.data_ptr(), out_type))
     return out

@@ -582,11 +582,24 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 1)
                     __threadfence();
 #pragma unroll
                     for (int c = 0; c < C; ++c) y[c] = 0.0f;
-                    for (int64_t cta = c0; cta <= c1; ++cta) {
-                        const int64_t b = first_unit(cta, p.units, ctas);
-                        const float* src = p.part + (2 * cta + (b >= t0 ? 0 : 1)) * (128 * BN);
+                    // (several CTAs' sums are on their way at once)
+                    constexpr int AHEAD = C > 32 ? 2 : (C > 16 ? 4 : 8);
+                    for (int64_t cta = c0; cta <= c1; cta += AHEAD) {
+                        float part[AHEAD][C];
 #pragma unroll
-                        for (int c = 0; c < C; ++c) y[c] += __ldcg(src + (half * C + c) * 128 + row);
+                        for (int j = 0; j < AHEAD; ++j) {
+                            const int64_t at = min(cta + j, c1);
+                            const int64_t b = first_unit(at, p.units, ctas);
+                            const float* src = p.part + (2 * at + (b >= t0 ? 0 : 1)) * (128 * BN);
+#pragma unroll
+                            for (int c = 0; c < C; ++c) part[j][c] = __ldcg(src + (half * C + c) * 128 + row);
+                        }
+#pragma unroll
+                        for (int j = 0; j < AHEAD; ++j) {
+                            if (cta + j > c1) break;
+#pragma unroll
+                            for (int c = 0; c < C; ++c) y[c] += part[j][c];
+                        }
                     }
                 }
             }
@@ -681,13 +694,17 @@ int few_width(int64_t M) {
     return bn <= 16 ? 16 : (bn <= 32 ? 32 : (bn <= 64 ? 64 : 128));
 }
 int64_t few_row_tiles(int64_t N) { return (N + 127) / 128; }
-int64_t few_ctas(int64_t M, int64_t N, int64_t K) {
-    const int64_t units = few_row_tiles(N) * few_tiles(M) * ((K + 127) / 128);
-    return units < sm_count() ? units : sm_count();
+// CTAs: one per SM, but at most 16 on a tile (each of a tile's CTAs costs its last
+// one about a tenth of a microsecond, a third of what a unit takes).
+constexpr int64_t kFewMaxCtas = 256;
+int64_t few_ctas(int64_t M, int64_t N, int64_t K, int64_t sms) {
+    const int64_t tiles = few_row_tiles(N) * few_tiles(M), units = tiles * ((K + 127) / 128);
+    const int64_t most = 16 * tiles < sms ? 16 * tiles : sms;
+    return units < most ? units : most;
 }
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
-    return round_up((size_t)few_ctas(M, N, K) * 2 * 128 * (size_t)few_width(M) * 4);
+    return round_up((size_t)few_ctas(M, N, K, kFewMaxCtas) * 2 * 128 * (size_t)few_width(M) * 4);
 }
 size_t few_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)few_row_tiles(N) * few_tiles(M) * 4); }
 
@@ -704,7 +721,8 @@ cudaError_t launch_few_t(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, 0, ready);
     if (e != cudaSuccess) return e;
-    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K)), Few<BN>::THREADS, smem, s);
+    const int64_t sms = sm_count() < kFewMaxCtas ? sm_count() : kFewMaxCtas;
+    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K, sms)), Few<BN>::THREADS, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
 }
 

@@ -60,7 +60,7 @@ class Fp8Blocks:
             raise ValueError("codes must be a float8_e4m3fn matrix")
         rows, cols = self.codes.shape
         want = (-(-rows // self.block_rows), -(-cols // FP8_BLOCK))
-        if self.scales.dtype != torch.float32 or tuple(self.scales.shape) != want:
+        if self.scales.dtype != torch.float32 or self.scales.shape != want:
             raise ValueError(f"scales must be float32 {list(want)}, one per block of {self.block_rows} x {FP8_BLOCK}")
 
     @property
@@ -70,6 +70,11 @@ class Fp8Blocks:
     def to(self, device: torch.device | str) -> Fp8Blocks:
         """Copy of this operand with both tensors on ``device``."""
         return Fp8Blocks(self.codes.to(device), self.scales.to(device), self.block_rows)
+
+
+def _flat(x: torch.Tensor) -> torch.Tensor:
+    """x [..., cols] as [rows, cols]."""
+    return x if x.ndim == 2 else x.reshape(x.shape[:-1].numel(), x.shape[-1])
 
 
 def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1) -> Fp8Blocks:
@@ -84,11 +89,7 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1) -> Fp8Blocks:
         raise ValueError("block_rows must be 1 or 128")
     if x.ndim < 1:
         raise ValueError("x must have shape [..., cols]")
-    flat = x.detach()
-    if flat.ndim != 2:
-        flat = flat.reshape(-1, flat.shape[-1]) if flat.shape[-1] else flat.reshape(flat.shape[:-1].numel(), 0)
-    codes, scales = _kernels.fp8_quantize(flat, block_rows)
-    return Fp8Blocks(codes, scales, block_rows)
+    return Fp8Blocks(*_kernels.fp8_quantize(_flat(x), block_rows), block_rows)
 
 
 def dequantize_fp8(q: Fp8Blocks, *, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -128,11 +129,8 @@ def fp8_gemm(
     if a.shape[-1] != n_in:
         raise ValueError(f"a has trailing dim {a.shape[-1]}, weight expects {n_in}")
     lead = a.shape[:-1]
-    flat = a.detach()
-    if flat.ndim != 2:
-        flat = flat.reshape(lead.numel(), n_in)
     dt = out_dtype if out_dtype is not None else (out.dtype if out is not None else a.dtype)
-    y = _kernels.fp8_gemm(flat, None, w.codes, w.scales, transpose, None if bias is None else bias.detach(), dt, out)
+    y = _kernels.fp8_gemm(_flat(a), None, w.codes, w.scales, transpose, bias, dt, out)
     return y if len(lead) == 1 else y.reshape(*lead, y.shape[1])
 
 
@@ -159,34 +157,31 @@ def fp8_weight_grad(
         raise ValueError("dy must have shape [..., out]")
     if accumulate and out is None:
         raise ValueError("accumulate adds to out, which is missing")
-    flat = dy.detach()
-    if flat.ndim != 2:
-        flat = flat.reshape(flat.shape[:-1].numel(), flat.shape[-1])
-    return _kernels.fp8_weight_grad(flat, x.codes, x.scales, out.dtype if out is not None else out_dtype, out,
+    return _kernels.fp8_weight_grad(_flat(dy), x.codes, x.scales, out.dtype if out is not None else out_dtype, out,
                                     accumulate)
 
 
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
-        xq = quantize_fp8(x)
-        wq = quantize_fp8(weight, block_rows=FP8_BLOCK)
-        y = _kernels.fp8_gemm(xq.codes, xq.scales, wq.codes, wq.scales, False, bias, x.dtype, None)
-        keep_x, keep_w = weight.requires_grad, x.requires_grad
-        ctx.save_for_backward(*((xq.codes, xq.scales) if keep_x else (None, None)),
-                              *((wq.codes, wq.scales) if keep_w else (None, None)))
+        xc, xs = _kernels.fp8_quantize(_flat(x), 1)
+        wc, ws = _kernels.fp8_quantize(weight, FP8_BLOCK)
+        y = _kernels.fp8_gemm(xc, xs, wc, ws, False, bias, x.dtype, None)
+        needs_x, needs_w, _ = ctx.needs_input_grad
+        ctx.save_for_backward(*((xc, xs) if needs_w else (None, None)), *((wc, ws) if needs_x else (None, None)))
         ctx.x_shape, ctx.x_dtype, ctx.w_dtype = x.shape, x.dtype, weight.dtype
         ctx.b_dtype = None if bias is None else bias.dtype
-        return y.reshape(*x.shape[:-1], weight.shape[0])
+        return y if x.ndim == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, dy: torch.Tensor) -> tuple[torch.Tensor | None, ...]:
         xc, xs, wc, ws = ctx.saved_tensors
-        dy2 = dy.reshape(dy.shape[:-1].numel(), dy.shape[-1])
+        dy2 = _flat(dy)
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
-            dx = _kernels.fp8_gemm(dy2, None, wc, ws, True, None, ctx.x_dtype, None).reshape(ctx.x_shape)
+            dx = _kernels.fp8_gemm(dy2, None, wc, ws, True, None, ctx.x_dtype, None)
+            dx = dx if len(ctx.x_shape) == 2 else dx.reshape(ctx.x_shape)
         if ctx.needs_input_grad[1]:
             dw = _kernels.fp8_weight_grad(dy2, xc, xs, ctx.w_dtype, None, False)
         if ctx.needs_input_grad[2]:
