@@ -192,6 +192,21 @@ def test_product_sizes(wq, cuda, K: int, N: int, transpose: bool) -> None:
         check_product(y, values64(a), w64 if transpose else w64.t(), bias, f"{rows}x{N}x{K}")
 
 
+@pytest.mark.parametrize("rows", [1, 20, 50, 128, 200])
+def test_product_long_runs(wq, cuda, rows: int) -> None:
+    """Large enough that every block's pipeline wraps around many times, called back to back without waiting."""
+    w = wq.quantize_fp8(rand((9000, 8000), 2, torch.bfloat16, 0.02), block_rows=128)
+    x = rand((rows, 8000), rows, torch.bfloat16)
+    prev = wq._kernels.set_fault_check(False)
+    try:
+        outs = [wq.fp8_gemm(x, w, out_dtype=torch.float32) for _ in range(6)]
+    finally:
+        wq._kernels.set_fault_check(prev)
+    assert wq._kernels.fault_status() == 0
+    check_product(outs[0], values64(wq.quantize_fp8(x)), values64(w).t())
+    assert all(torch.equal(y, outs[0]) for y in outs)
+
+
 @pytest.mark.parametrize("rows", [1, 4, 17, 64, 150, 600])
 def test_product_of_a_tensor_equals_quantize_then_product(wq, cuda, rows: int) -> None:
     w = wq.quantize_fp8(rand((700, 1030), 2, scale=0.02), block_rows=128)

@@ -319,18 +319,25 @@ struct Few {
     static constexpr int SUM_WARPS = BN > 64 ? 8 : 4;
     static constexpr int COLS = BN > 64 ? BN / 2 : BN;          // columns per summing warp
     static constexpr int THREADS = 128 + 32 * SUM_WARPS;
-    static constexpr int BUFS = BN > 64 ? 4 : 8;                // even: each issuing warp has its own
-    static constexpr uint32_t TMEM = BUFS * BN;
     static constexpr int STAGE = kOperandBytes + BN * 128;
-    static constexpr int STAGES = (BN > 64 ? 192 : 200) * 1024 / STAGE / 2 * 2;   // even likewise
+    // With few columns two CTAs share an SM: one's beginning and end (the first loads,
+    // the partial sums) run beside the other's stream.
+    static constexpr int CTAS = BN > 32 ? 1 : 2;
+    static constexpr int STAGES = (BN > 64 ? 192 : 206) * 1024 / CTAS / STAGE / 2 * 2;   // even likewise
+    // Tensor-memory buffers: even, and no more than stages: a stage's barrier must not
+    // complete twice before the summing warps have seen it once.
+    static constexpr int BUFS = BN > 64 ? 4 : (STAGES < 8 ? STAGES : 8);
+    static_assert(BUFS <= STAGES, "a stage's barrier would lap the summing warps");
+    static constexpr uint32_t TMEM = BUFS * BN;
     static constexpr int SCALES = STAGES * STAGE;               // per buffer BN of a, one of w
     static constexpr int SCALE_BYTES = (BN + 4) * 4;
     static constexpr int BAR = SCALES + BUFS * SCALE_BYTES;
     // full, done per stage; scales there, sums empty per buffer
     static constexpr int TMEM_SLOT = BAR + 8 * (2 * STAGES + 2 * BUFS);
+    static_assert((TMEM & (TMEM - 1)) == 0 && TMEM >= 32 && TMEM * CTAS <= 512, "tensor memory is handed out in powers of two");
     static constexpr int FLAG = TMEM_SLOT + 8;
     static constexpr int TOTAL = TMEM_SLOT + 16;
-    static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
+    static_assert((TOTAL + 1024 + 1024) * CTAS <= 228 * 1024, "stages exceed the shared memory of an SM");
 };
 
 struct FewParams {
@@ -358,7 +365,7 @@ __device__ __forceinline__ int64_t cta_of(int64_t unit, int64_t units, int64_t c
 }
 
 template <int BN, bool WT>
-__global__ void __launch_bounds__(Few<BN>::THREADS, 1)
+__global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
     fp8_gemm_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap map_a,
                         const __grid_constant__ CUtensorMap map_w) {
     using L = Few<BN>;
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 1)
         };
         // the first round's weights may come before the previous kernel (which makes
         // a's codes) is over
-        const int ahead = (int)min((int64_t)NS, u1 - u0);
+        const int ahead = p.weights_ready ? (int)min((int64_t)NS, u1 - u0) : 0;
         {
             int t = tile, c = b;
             for (int s = 0; s < ahead; ++s) {
@@ -583,22 +590,24 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < C; ++c) y[c] = 0.0f;
                     // (several CTAs' sums are on their way at once)
-                    constexpr int AHEAD = C > 32 ? 2 : (C > 16 ? 4 : 8);
+                    constexpr int AHEAD = C > 32 ? 1 : (C > 16 ? 2 : 4);
                     for (int64_t cta = c0; cta <= c1; cta += AHEAD) {
                         float part[AHEAD][C];
 #pragma unroll
                         for (int j = 0; j < AHEAD; ++j) {
-                            const int64_t at = min(cta + j, c1);
-                            const int64_t b = first_unit(at, p.units, ctas);
-                            const float* src = p.part + (2 * at + (b >= t0 ? 0 : 1)) * (128 * BN);
+                            if (cta + j <= c1) {
+                                const int64_t b = first_unit(cta + j, p.units, ctas);
+                                const float* src = p.part + (2 * (cta + j) + (b >= t0 ? 0 : 1)) * (128 * BN);
 #pragma unroll
-                            for (int c = 0; c < C; ++c) part[j][c] = __ldcg(src + (half * C + c) * 128 + row);
+                                for (int c = 0; c < C; ++c) part[j][c] = __ldcg(src + (half * C + c) * 128 + row);
+                            }
                         }
 #pragma unroll
                         for (int j = 0; j < AHEAD; ++j) {
-                            if (cta + j > c1) break;
+                            if (cta + j <= c1) {
 #pragma unroll
-                            for (int c = 0; c < C; ++c) y[c] += part[j][c];
+                                for (int c = 0; c < C; ++c) y[c] += part[j][c];
+                            }
                         }
                     }
                 }
@@ -694,12 +703,12 @@ int few_width(int64_t M) {
     return bn <= 16 ? 16 : (bn <= 32 ? 32 : (bn <= 64 ? 64 : 128));
 }
 int64_t few_row_tiles(int64_t N) { return (N + 127) / 128; }
-// CTAs: one per SM, but at most 16 on a tile (each of a tile's CTAs costs its last
+// CTAs: as many as are resident, but at most 16 on a tile (each of a tile's CTAs costs its last
 // one about a tenth of a microsecond, a third of what a unit takes).
-constexpr int64_t kFewMaxCtas = 256;
-int64_t few_ctas(int64_t M, int64_t N, int64_t K, int64_t sms) {
+constexpr int64_t kFewMaxCtas = 512;
+int64_t few_ctas(int64_t M, int64_t N, int64_t K, int64_t resident) {
     const int64_t tiles = few_row_tiles(N) * few_tiles(M), units = tiles * ((K + 127) / 128);
-    const int64_t most = 16 * tiles < sms ? 16 * tiles : sms;
+    const int64_t most = 16 * tiles < resident ? 16 * tiles : resident;
     return units < most ? units : most;
 }
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -721,8 +730,8 @@ cudaError_t launch_few_t(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, 0, ready);
     if (e != cudaSuccess) return e;
-    const int64_t sms = sm_count() < kFewMaxCtas ? sm_count() : kFewMaxCtas;
-    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K, sms)), Few<BN>::THREADS, smem, s);
+    const int64_t resident = (int64_t)sm_count() * Few<BN>::CTAS;
+    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K, resident < kFewMaxCtas ? resident : kFewMaxCtas)), Few<BN>::THREADS, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
 }
 
