@@ -348,7 +348,6 @@ struct FewParams {
     const void* bias;
     int bias_type;
     void* out;
-    int out_type;
     int64_t ldo;
     int M, N, blocks;
     int tiles_a, bn;         // tiles of bn rows of a
@@ -364,7 +363,7 @@ __device__ __forceinline__ int64_t cta_of(int64_t unit, int64_t units, int64_t c
     return ((unit + 1) * ctas - 1) / units;
 }
 
-template <int BN, bool WT>
+template <int BN, bool WT, typename O>
 __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
     fp8_gemm_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap map_a,
                         const __grid_constant__ CUtensorMap map_w) {
@@ -541,8 +540,8 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                 const float w = sc[BN];
                 const uint64_t w2 = pack2(w, w);
 #pragma unroll
-                for (int c0 = 0; c0 < C; c0 += (C < 32 ? C : 32)) {
-                    constexpr int STEP = C < 32 ? C : 32;
+                for (int c0 = 0; c0 < C; c0 += C) {
+                    constexpr int STEP = C;
                     uint64_t v[STEP / 2];
                     tmem_pairs(taddr + (uint32_t)(buf * BN + c0), v);
 #pragma unroll
@@ -564,19 +563,21 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                     bph ^= 1u;
                 }
             }
-            float y[C];
+            float4 y[C / 4];
 #pragma unroll
-            for (int c = 0; c < C / 2; ++c) {
-                const float2 f = unpack2(acc[c]);
-                y[2 * c] = f.x;
-                y[2 * c + 1] = f.y;
+            for (int c = 0; c < C / 4; ++c) {
+                const float2 f = unpack2(acc[2 * c]), g = unpack2(acc[2 * c + 1]);
+                y[c] = make_float4(f.x, f.y, g.x, g.y);
             }
             bool write = true;
             if (from != t0 || to != t1) {
+                // slot [column / 4][row][4]: 16 bytes per lane, lanes side by side
                 const int64_t ctas = gridDim.x;
-                float* mine = p.part + (2 * (int64_t)blockIdx.x + (from == u0 ? 0 : 1)) * (128 * BN);
+                const int64_t lane_at = (half * (C / 4) * 128 + row) * 4;
+                float4* mine = reinterpret_cast<float4*>(
+                    p.part + (2 * (int64_t)blockIdx.x + (from == u0 ? 0 : 1)) * (128 * BN) + lane_at);
 #pragma unroll
-                for (int c = 0; c < C; ++c) mine[(half * C + c) * 128 + row] = y[c];
+                for (int c = 0; c < C / 4; ++c) mine[c * 128] = y[c];
                 __threadfence();
                 named_barrier(1, 32 * L::SUM_WARPS);
                 volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
@@ -588,25 +589,32 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                 if (write) {
                     __threadfence();
 #pragma unroll
-                    for (int c = 0; c < C; ++c) y[c] = 0.0f;
+                    for (int c = 0; c < C / 4; ++c) y[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     // (several CTAs' sums are on their way at once)
-                    constexpr int AHEAD = C > 32 ? 1 : (C > 16 ? 2 : 4);
+                    constexpr int AHEAD = C > 16 ? 1 : 3;
+#pragma unroll 1
                     for (int64_t cta = c0; cta <= c1; cta += AHEAD) {
-                        float part[AHEAD][C];
+                        float4 part[AHEAD][C / 4];
 #pragma unroll
                         for (int j = 0; j < AHEAD; ++j) {
                             if (cta + j <= c1) {
                                 const int64_t b = first_unit(cta + j, p.units, ctas);
-                                const float* src = p.part + (2 * (cta + j) + (b >= t0 ? 0 : 1)) * (128 * BN);
+                                const float4* src = reinterpret_cast<const float4*>(
+                                    p.part + (2 * (cta + j) + (b >= t0 ? 0 : 1)) * (128 * BN) + lane_at);
 #pragma unroll
-                                for (int c = 0; c < C; ++c) part[j][c] = __ldcg(src + (half * C + c) * 128 + row);
+                                for (int c = 0; c < C / 4; ++c) part[j][c] = __ldcg(src + c * 128);
                             }
                         }
 #pragma unroll
                         for (int j = 0; j < AHEAD; ++j) {
                             if (cta + j <= c1) {
 #pragma unroll
-                                for (int c = 0; c < C; ++c) y[c] += part[j][c];
+                                for (int c = 0; c < C / 4; ++c) {
+                                    y[c].x += part[j][c].x;
+                                    y[c].y += part[j][c].y;
+                                    y[c].z += part[j][c].z;
+                                    y[c].w += part[j][c].w;
+                                }
                             }
                         }
                     }
@@ -617,15 +625,13 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                 const float bias = load_any(p.bias, p.bias_type, n);
                 const int m0 = tile % p.tiles_a * p.bn + half * C;
                 const int cols = min(C, min(p.bn - half * C, p.M - m0));
-                const int64_t at = m0 * p.ldo + n;
+                O* at = static_cast<O*>(p.out) + m0 * p.ldo + n;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    if (c < cols) {
-                        const float v = y[c] + bias;
-                        if (p.out_type == kBf16) static_cast<__nv_bfloat16*>(p.out)[at + c * p.ldo] = from_f32<__nv_bfloat16>(v);
-                        else if (p.out_type == kF16) static_cast<__half*>(p.out)[at + c * p.ldo] = from_f32<__half>(v);
-                        else static_cast<float*>(p.out)[at + c * p.ldo] = v;
-                    }
+                    const float4 f = y[c / 4];
+                    const float v = c % 4 == 0 ? f.x : (c % 4 == 1 ? f.y : (c % 4 == 2 ? f.z : f.w));
+                    if (c < cols) *at = from_f32<O>(v + bias);
+                    at += p.ldo;
                 }
             }
         }
@@ -703,13 +709,15 @@ int few_width(int64_t M) {
     return bn <= 16 ? 16 : (bn <= 32 ? 32 : (bn <= 64 ? 64 : 128));
 }
 int64_t few_row_tiles(int64_t N) { return (N + 127) / 128; }
-// CTAs: as many as are resident, but at most 16 on a tile (each of a tile's CTAs costs its last
-// one about a tenth of a microsecond, a third of what a unit takes).
-constexpr int64_t kFewMaxCtas = 512;
+// CTAs: as many as are resident, but with runs of six units and more (a shared tile
+// costs two to four microseconds, a unit a third of one), and at most 16 on a tile.
+constexpr int64_t kFewMaxCtas = 512, kFewRun = 6;
 int64_t few_ctas(int64_t M, int64_t N, int64_t K, int64_t resident) {
     const int64_t tiles = few_row_tiles(N) * few_tiles(M), units = tiles * ((K + 127) / 128);
-    const int64_t most = 16 * tiles < resident ? 16 * tiles : resident;
-    return units < most ? units : most;
+    int64_t n = (units + kFewRun - 1) / kFewRun;
+    if (n < tiles) n = tiles;
+    if (n > 16 * tiles) n = 16 * tiles;
+    return n < resident ? n : resident;
 }
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
@@ -719,20 +727,27 @@ size_t few_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)few_row
 
 bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= 128; }
 
-template <int BN, bool WT>
-cudaError_t launch_few_t(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
+template <int BN, bool WT, typename O>
+cudaError_t launch_few_o(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
     CUtensorMap ma, mw;
     if (!encode_codes(&ma, g.a.codes, g.a.cols, g.a.rows, g.a.ld, (uint32_t)p.bn) ||
         !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, 128))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)Few<BN>::TOTAL + 1024;
-    auto kern = fp8_gemm_few_kernel<BN, WT>;
+    auto kern = fp8_gemm_few_kernel<BN, WT, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, 0, ready);
     if (e != cudaSuccess) return e;
     const int64_t resident = (int64_t)sm_count() * Few<BN>::CTAS;
     LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K, resident < kFewMaxCtas ? resident : kFewMaxCtas)), Few<BN>::THREADS, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
+}
+
+template <int BN, bool WT>
+cudaError_t launch_few_t(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
+    if (g.out_type == kF16) return launch_few_o<BN, WT, __half>(g, p, s);
+    if (g.out_type == kBf16) return launch_few_o<BN, WT, __nv_bfloat16>(g, p, s);
+    return launch_few_o<BN, WT, float>(g, p, s);
 }
 
 template <bool WT>
@@ -747,7 +762,6 @@ cudaError_t launch_few(const Fp8Gemm& g, void* workspace, bool prepared, cudaStr
     p.bias = g.bias;
     p.bias_type = g.bias_type;
     p.out = g.out;
-    p.out_type = g.out_type;
     p.ldo = g.ldo;
     p.M = (int)g.M;
     p.N = (int)g.N;
