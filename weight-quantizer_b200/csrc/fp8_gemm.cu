@@ -45,6 +45,7 @@ struct PairSmem {
     // full and done per stage (done: the block's MMAs are over, so its operands
     // may be replaced and its sums read); sums empty[2]
     static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 2);
+    static constexpr int FLAG = TMEM_SLOT + 8;
     static constexpr int TOTAL = TMEM_SLOT + 16;
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
 };
@@ -62,6 +63,9 @@ struct PairParams {
     int M, N, blocks;        // inner blocks of 128
     int tiles_m, tiles_n, band;
     bool wide_out;           // rows of out are 32-byte aligned
+    int splits;              // parts of the inner blocks, each a tile's work for a pair of its own
+    float* part;             // [tile][split][rank] sums of 128 x 256
+    unsigned int* arrived;   // [tile][rank], zeroed before the launch
     unsigned int* fault;
 };
 
@@ -108,7 +112,7 @@ __device__ __forceinline__ void store32(O* row, int64_t c, int64_t n, bool wide,
     }
 }
 
-template <bool WT>
+template <bool WT, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     fp8_gemm_pair_kernel(const PairParams p, const __grid_constant__ CUtensorMap map_a,
                          const __grid_constant__ CUtensorMap map_w) {
@@ -141,9 +145,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     grid_wait();   // nothing above reads global memory
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_SLOT);
     const int pairs = (int)gridDim.x >> 1, first = (int)blockIdx.x >> 1;
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int mine = first < tiles ? (tiles - 1 - first) / pairs + 1 : 0;
-    const int64_t steps = (int64_t)mine * p.blocks;
+    // items of work: tiles, or parts of their inner blocks
+    const int splits = SPLIT ? p.splits : 1;
+    const int items = p.tiles_m * p.tiles_n * splits;
+    auto from_block = [&](int item) { return SPLIT ? item % splits * p.blocks / splits : 0; };
+    auto to_block = [&](int item) { return SPLIT ? (item % splits + 1) * p.blocks / splits : p.blocks; };
+    int64_t steps = 0;
+    for (int i = first; i < items; i += pairs) steps += to_block(i) - from_block(i);
     bool faulted = false;
     auto give_up = [&]() {
         faulted = true;
@@ -158,11 +166,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             const uint32_t full0 = in_cta(full(0), 0);
             int s = 0;
             uint32_t ph = 1;
-            for (int t = first; t < tiles; t += pairs) {
+            for (int t = first; t < items; t += pairs) {
                 int mt, nt;
-                tile_of(t, p, mt, nt);
+                tile_of(t / splits, p, mt, nt);
                 const int m0 = mt * kPairTile + rank * 128, n0 = nt * kPairTile + rank * 128;
-                for (int b = 0; b < p.blocks; ++b) {
+                const int b1 = to_block(t);
+                for (int b = from_block(t); b < b1; ++b) {
                     if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
                     __syncwarp();
                     if (elect_one()) {
@@ -229,9 +238,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         int64_t i = 0;
         int s = 0;
         uint32_t ph = 0;
-        for (int t = first; t < tiles; t += pairs) {
+        for (int t = first; t < items; t += pairs) {
             int mt, nt;
-            tile_of(t, p, mt, nt);
+            tile_of(t / splits, p, mt, nt);
+            const int b0 = from_block(t), b1 = to_block(t);
             const int64_t m = (int64_t)mt * kPairTile + rank * 128 + q * 32 + lane;
             const int64_t n0 = (int64_t)nt * kPairTile + half * 128;
             const float* sa = p.sa + min(m, (int64_t)p.M - 1) * p.sa_row;
@@ -240,14 +250,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
             for (int c = 0; c < 64; ++c) acc[c] = 0;
             // the scales of the next three blocks are on their way
+            sa += b0 * p.sa_col, sw += b0 * p.sw_k;
             float a1 = __ldg(sa), w1 = __ldg(sw), a2 = 0, w2 = 0, a3 = 0, w3 = 0;
-            if (p.blocks > 1) a2 = __ldg(sa + p.sa_col), w2 = __ldg(sw + p.sw_k);
-            if (p.blocks > 2) a3 = __ldg(sa + 2 * p.sa_col), w3 = __ldg(sw + 2 * p.sw_k);
-            for (int b = 0; b < p.blocks; ++b, ++i) {
+            if (b0 + 1 < b1) a2 = __ldg(sa + p.sa_col), w2 = __ldg(sw + p.sw_k);
+            if (b0 + 2 < b1) a3 = __ldg(sa + 2 * p.sa_col), w3 = __ldg(sw + 2 * p.sw_k);
+            for (int b = 0; b < b1 - b0; ++b, ++i) {
                 const int buf = (int)(i & 1);
                 const float sc = a1 * w1;
                 a1 = a2, w1 = w2, a2 = a3, w2 = w3;
-                if (b + 3 < p.blocks) a3 = __ldg(sa + (b + 3) * p.sa_col), w3 = __ldg(sw + (b + 3) * p.sw_k);
+                if (b + 3 < b1 - b0) a3 = __ldg(sa + (b + 3) * p.sa_col), w3 = __ldg(sw + (b + 3) * p.sw_k);
                 const uint64_t sc2 = pack2(sc, sc);
                 const uint32_t from = taddr + (uint32_t)(buf * 256);
                 uint64_t v[32];
@@ -268,7 +279,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     ph ^= 1u;
                 }
             }
-            if (m < p.M) {
+            bool write = true;
+            if constexpr (SPLIT) {
+                // the item's sums go to its slot, [column / 4][row][4]; the last of the
+                // tile's items adds them in order
+                const int64_t lane_at = ((int64_t)half * 32 * 128 + q * 32 + lane) * 4;
+                constexpr int64_t SLOT = 128 * 256;
+                float4* mine = reinterpret_cast<float4*>(p.part + ((int64_t)t * 2 + rank) * SLOT + lane_at);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    const float2 f = unpack2(acc[2 * c]), g = unpack2(acc[2 * c + 1]);
+                    mine[c * 128] = make_float4(f.x, f.y, g.x, g.y);
+                }
+                __threadfence();
+                named_barrier(1, 256);
+                volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
+                const int tile = t / splits;
+                if (warp == 4 && lane == 0)
+                    *flag = atomicAdd(p.arrived + tile * 2 + rank, 1u) == (unsigned)(splits - 1);
+                named_barrier(1, 256);
+                write = *flag != 0u;
+                named_barrier(1, 256);   // the flag has been read
+                if (write) {
+                    __threadfence();
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) acc[c] = 0;
+                    const uint64_t one = pack2(1.0f, 1.0f);
+#pragma unroll 1
+                    for (int sp = 0; sp < splits; ++sp) {
+                        const float4* src = reinterpret_cast<const float4*>(
+                            p.part + (((int64_t)tile * splits + sp) * 2 + rank) * SLOT + lane_at);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const float4 f = __ldcg(src + c * 128);
+                            fma2(acc[2 * c], pack2(f.x, f.y), one);
+                            fma2(acc[2 * c + 1], pack2(f.z, f.w), one);
+                        }
+                    }
+                }
+            }
+            if (write && m < p.M) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float v[32];
@@ -316,17 +366,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 template <int BN>
 struct Few {
-    static constexpr int SUM_WARPS = BN > 64 ? 8 : 4;
-    static constexpr int COLS = BN > 64 ? BN / 2 : BN;          // columns per summing warp
+    static constexpr int COLS = BN < 32 ? BN : 32;              // columns per summing warp
+    static constexpr int SUM_WARPS = 4 * (BN / COLS);
     static constexpr int THREADS = 128 + 32 * SUM_WARPS;
     static constexpr int STAGE = kOperandBytes + BN * 128;
     // With few columns two CTAs share an SM: one's beginning and end (the first loads,
     // the partial sums) run beside the other's stream.
     static constexpr int CTAS = BN > 32 ? 1 : 2;
-    static constexpr int STAGES = (BN > 64 ? 192 : 206) * 1024 / CTAS / STAGE / 2 * 2;   // even likewise
+    static constexpr int STAGES = 206 * 1024 / CTAS / STAGE / 2 * 2;   // even likewise
     // Tensor-memory buffers: even, and no more than stages: a stage's barrier must not
     // complete twice before the summing warps have seen it once.
-    static constexpr int BUFS = BN > 64 ? 4 : (STAGES < 8 ? STAGES : 8);
+    static constexpr int BUFS = STAGES < 8 ? STAGES : 8;
     static_assert(BUFS <= STAGES, "a stage's barrier would lap the summing warps");
     static constexpr uint32_t TMEM = BUFS * BN;
     static constexpr int SCALES = STAGES * STAGE;               // per buffer BN of a, one of w
@@ -350,7 +400,7 @@ struct FewParams {
     void* out;
     int64_t ldo;
     int M, N, blocks;
-    int tiles_a, bn;         // tiles of bn rows of a
+    int bn;                  // rows of a in the MMA: M in steps of 16
     int64_t units;
     float* part;             // two slots of 128 x BN sums per CTA
     unsigned int* arrived;   // per tile, zeroed before the launch
@@ -410,13 +460,13 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
         const uint32_t bytes = (uint32_t)(kOperandBytes + p.bn * 128);
         int tile = (int)(u0 / p.blocks), b = (int)(u0 - (int64_t)tile * p.blocks);
         auto load_w = [&](int s, int tile, int b) {
-            const int r0 = tile / p.tiles_a * 128;
+            const int r0 = tile * 128;
             mbar_arrive_expect_tx(full(s), bytes);
             if constexpr (WT) tma_box<1>(sbase + (uint32_t)(s * L::STAGE), &map_w, r0, b * 128, full(s));
             else tma_box<1>(sbase + (uint32_t)(s * L::STAGE), &map_w, b * 128, r0, full(s));
         };
-        auto load_a = [&](int s, int tile, int b) {
-            tma_box<1>(sbase + (uint32_t)(s * L::STAGE + kOperandBytes), &map_a, b * 128, tile % p.tiles_a * p.bn, full(s));
+        auto load_a = [&](int s, int b) {
+            tma_box<1>(sbase + (uint32_t)(s * L::STAGE + kOperandBytes), &map_a, b * 128, 0, full(s));
         };
         // the first round's weights may come before the previous kernel (which makes
         // a's codes) is over
@@ -438,7 +488,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
             __syncwarp();
             if (elect_one()) {
                 if (!loaded) load_w(s, tile, b);
-                load_a(s, tile, b);
+                load_a(s, b);
             }
             __syncwarp();
             if (++b == p.blocks) b = 0, ++tile;
@@ -496,15 +546,14 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
         for (int64_t u = u0; u < u1; ++u) {
             wait(sums_empty(buf), bph);
             __syncwarp();
-            const int m0 = tile % p.tiles_a * p.bn;
             const uint32_t to = sbase + (uint32_t)(L::SCALES + buf * L::SCALE_BYTES);
 #pragma unroll
             for (int i = 0; i < (BN + 31) / 32; ++i) {
                 const int c = i * 32 + lane;
-                const bool some = c < p.bn && m0 + c < p.M;
-                if (c < BN) cp_async4_s(to + c * 4, some ? p.sa + (m0 + c) * p.sa_row + b * p.sa_col : p.sa, some);
+                const bool some = c < p.M;
+                if (c < BN) cp_async4_s(to + c * 4, some ? p.sa + c * p.sa_row + b * p.sa_col : p.sa, some);
             }
-            if (lane == 0) cp_async4_s(to + BN * 4, p.sw + tile / p.tiles_a * p.sw_n + b * p.sw_k, true);
+            if (lane == 0) cp_async4_s(to + BN * 4, p.sw + tile * p.sw_n + b * p.sw_k, true);
             cp_async_arrive(scaled(buf));
             if (++b == p.blocks) b = 0, ++tile;
             if (++buf == NB) {
@@ -539,18 +588,17 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                 const float* sc = reinterpret_cast<const float*>(smem + L::SCALES + buf * L::SCALE_BYTES);
                 const float w = sc[BN];
                 const uint64_t w2 = pack2(w, w);
+                uint64_t by[C / 2];
 #pragma unroll
-                for (int c0 = 0; c0 < C; c0 += C) {
-                    constexpr int STEP = C;
-                    uint64_t v[STEP / 2];
-                    tmem_pairs(taddr + (uint32_t)(buf * BN + c0), v);
-#pragma unroll
-                    for (int c = 0; c < STEP / 4; ++c) {
-                        const float4 f = *reinterpret_cast<const float4*>(sc + half * C + c0 + 4 * c);
-                        fma2(acc[c0 / 2 + 2 * c], v[2 * c], mul2(pack2(f.x, f.y), w2));
-                        fma2(acc[c0 / 2 + 2 * c + 1], v[2 * c + 1], mul2(pack2(f.z, f.w), w2));
-                    }
+                for (int c = 0; c < C / 4; ++c) {
+                    const float4 f = *reinterpret_cast<const float4*>(sc + half * C + 4 * c);
+                    by[2 * c] = mul2(pack2(f.x, f.y), w2);
+                    by[2 * c + 1] = mul2(pack2(f.z, f.w), w2);
                 }
+                uint64_t v[C / 2];
+                tmem_pairs(taddr + (uint32_t)(buf * BN), v);
+#pragma unroll
+                for (int c = 0; c < C / 2; ++c) fma2(acc[c], v[c], by[c]);
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sums_empty(buf));
@@ -620,12 +668,11 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                     }
                 }
             }
-            const int n = tile / p.tiles_a * 128 + row;
+            const int n = tile * 128 + row;
             if (write && n < p.N) {
                 const float bias = load_any(p.bias, p.bias_type, n);
-                const int m0 = tile % p.tiles_a * p.bn + half * C;
-                const int cols = min(C, min(p.bn - half * C, p.M - m0));
-                O* at = static_cast<O*>(p.out) + m0 * p.ldo + n;
+                const int cols = min(C, p.M - half * C);
+                O* at = static_cast<O*>(p.out) + (int64_t)half * C * p.ldo + n;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     const float4 f = y[c / 4];
@@ -653,8 +700,32 @@ __global__ void fill_rows_kernel(O* out, int64_t M, int64_t N, int64_t ldo, cons
         out[i / N * ldo + i % N] = from_f32<O>(load_any(bias, bias_type, i % N));
 }
 
-template <bool WT>
-cudaError_t launch_pair(const Fp8Gemm& g, cudaStream_t s) {
+// ---- plan ----
+
+size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
+int64_t pair_tiles(int64_t M, int64_t N) {
+    return ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile);
+}
+// Few tiles (at most half as many as pairs of SMs): their inner blocks are cut into
+// parts of at least four, one pair each, where that saves more than the parts' sums
+// cost (16 + 2 each, in microseconds, at 0.43 per block: 129 x 4096 x 11008 in four
+// parts 31, whole 37; 129 x 4096 x 4096 in four parts 24, whole 18).
+constexpr int64_t kPairMaxSplits = 8;
+int pair_splits(int64_t M, int64_t N, int64_t K) {
+    const int64_t tiles = pair_tiles(M, N), blocks = (K + 127) / 128;
+    int64_t n = sm_count() / 2 / tiles;
+    if (n > blocks / 4) n = blocks / 4;
+    if (n > kPairMaxSplits) n = kPairMaxSplits;
+    if (n < 2 || 0.43 * (double)(blocks - (blocks + n - 1) / n) < 16.0 + 2.0 * (double)n) return 1;
+    return (int)n;
+}
+size_t pair_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)pair_tiles(M, N) * 2 * 4); }
+size_t pair_part_bytes(int64_t M, int64_t N, int64_t K) {
+    return (size_t)pair_tiles(M, N) * pair_splits(M, N, K) * 2 * 128 * 256 * 4;
+}
+
+template <bool WT, bool SPLIT>
+cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
     PairParams p;
     p.sa = g.a.scales;
     p.sa_row = g.a.s_row;
@@ -679,6 +750,10 @@ cudaError_t launch_pair(const Fp8Gemm& g, cudaStream_t s) {
     const int64_t bands = (p.tiles_m + band - 1) / band;
     p.band = (int)((p.tiles_m + bands - 1) / bands);
     p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * type_bytes(g.out_type)) % 32 == 0;
+    p.splits = splits;
+    p.arrived = static_cast<unsigned int*>(workspace);
+    p.part = SPLIT ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pair_arrived_bytes(g.M, g.N))
+                   : nullptr;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
     CUtensorMap ma, mw;
@@ -686,46 +761,73 @@ cudaError_t launch_pair(const Fp8Gemm& g, cudaStream_t s) {
         !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, 128))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)PairSmem::TOTAL + 1024;
-    auto kern = fp8_gemm_pair_kernel<WT>;
+    auto kern = fp8_gemm_pair_kernel<WT, SPLIT>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kPairLaunchRegs, ready);
     if (e != cudaSuccess) return e;
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int pairs = sm_count() / 2;
-    LaunchConfig cfg(dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), kPairThreads, smem, s);
+    const int64_t items = (int64_t)p.tiles_m * p.tiles_n * splits;
+    const int64_t pairs = sm_count() / 2;
+    if (items > 0x7fffffff) return cudaErrorInvalidValue;
+    LaunchConfig cfg(dim3(2u * (unsigned)(items < pairs ? items : pairs)), kPairThreads, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
+}
+
+template <bool WT>
+cudaError_t launch_pair(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
+    const int splits = pair_splits(g.M, g.N, g.K);
+    if (splits == 1) return launch_pair_s<WT, false>(g, 1, nullptr, s);
+    if (!prepared) {
+        cudaError_t e = cudaMemsetAsync(workspace, 0, pair_arrived_bytes(g.M, g.N), s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pair_s<WT, true>(g, splits, workspace, s);
 }
 
 // ---- few rows: plan ----
 
-// Tiles of a's rows: as few as hold at most 128 each, of equal size in steps of 16.
-int few_tiles(int64_t M) { return (int)((M + 127) / 128); }
-int few_bn(int64_t M) {
-    const int64_t t = few_tiles(M);
-    return (int)(((M + t - 1) / t + 15) / 16 * 16);
-}
-int few_width(int64_t M) {
-    const int bn = few_bn(M);
-    return bn <= 16 ? 16 : (bn <= 32 ? 32 : (bn <= 64 ? 64 : 128));
-}
-int64_t few_row_tiles(int64_t N) { return (N + 127) / 128; }
+constexpr int kFewMaxRows = 64;
+int few_bn(int64_t M) { return (int)((M + 15) / 16 * 16); }
+int few_width(int64_t M) { return M <= 16 ? 16 : (M <= 32 ? 32 : 64); }
+int64_t few_tiles(int64_t N) { return (N + 127) / 128; }
 // CTAs: as many as are resident, but with runs of six units and more (a shared tile
-// costs two to four microseconds, a unit a third of one), and at most 16 on a tile.
+// costs two to four microseconds, a unit half of one), and at most 16 on a tile.
 constexpr int64_t kFewMaxCtas = 512, kFewRun = 6;
-int64_t few_ctas(int64_t M, int64_t N, int64_t K, int64_t resident) {
-    const int64_t tiles = few_row_tiles(N) * few_tiles(M), units = tiles * ((K + 127) / 128);
+int64_t few_ctas(int64_t N, int64_t K, int64_t resident) {
+    const int64_t tiles = few_tiles(N), units = tiles * ((K + 127) / 128);
     int64_t n = (units + kFewRun - 1) / kFewRun;
     if (n < tiles) n = tiles;
     if (n > 16 * tiles) n = 16 * tiles;
     return n < resident ? n : resident;
 }
-size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
-size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
-    return round_up((size_t)few_ctas(M, N, K, kFewMaxCtas) * 2 * 128 * (size_t)few_width(M) * 4);
+int64_t few_resident(int64_t M) {
+    const int64_t n = (int64_t)sm_count() * (M <= 32 ? 2 : 1);
+    return n < kFewMaxCtas ? n : kFewMaxCtas;
 }
-size_t few_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)few_row_tiles(N) * few_tiles(M) * 4); }
+size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
+    return round_up((size_t)few_ctas(N, K, kFewMaxCtas) * 2 * 128 * (size_t)few_width(M) * 4);
+}
+size_t few_arrived_bytes(int64_t N) { return round_up((size_t)few_tiles(N) * 4); }
 
-bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= 128; }
+// Which of the two kernels: the shorter by this model, in microseconds, fitted to
+// both on weights of 2304 x 768 to 28672 x 8192 at 1 to 128 rows (from memory, not
+// L2). Pairs: 5, and 0.43 for each round of blocks, or the weights at 5.5 TB/s if
+// that is longer; parts of tiles cost 12 + 2 each. Few rows: 8, a unit's time for
+// each unit of a CTA's run, and the CTAs that share a tile. Measured, pairs / few:
+// 28672 x 8192 at 16 rows 60 / 48, at 64 rows 66 / 58, at 128 rows 69 / 78;
+// 11008 x 4096 at 64 rows 19 / 25; 4096 x 11008 at 64 rows 31 / 24; 2304 x 768 6 / 8.
+double pair_us(int64_t M, int64_t N, int64_t K) {
+    const int64_t s = pair_splits(M, N, K), pairs = sm_count() / 2, blocks = (K + 127) / 128;
+    const double rounds = (double)((pair_tiles(M, N) * s + pairs - 1) / pairs);
+    const double run = rounds * (double)((blocks + s - 1) / s) * 0.43, stream = (double)N * (double)K / 5.5e6;
+    return 5.0 + (run > stream ? run : stream) + (s > 1 ? 12.0 + 2.0 * (double)s : 0.0);
+}
+double few_us(int64_t M, int64_t N, int64_t K) {
+    const int64_t blocks = (K + 127) / 128, units = few_tiles(N) * blocks;
+    const double run = (double)units / (double)few_ctas(N, K, few_resident(M));
+    const double shared = (double)blocks / run;   // CTAs on a tile
+    return 8.0 + run * (M <= 32 ? 0.86 : 0.54) + (shared > 1.0 ? shared * (M <= 16 ? 0.5 : (M <= 32 ? 0.7 : 1.2)) : 0.0);
+}
+bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kFewMaxRows && few_us(M, N, K) <= pair_us(M, N, K); }
 
 template <int BN, bool WT, typename O>
 cudaError_t launch_few_o(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
@@ -738,8 +840,8 @@ cudaError_t launch_few_o(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, 0, ready);
     if (e != cudaSuccess) return e;
-    const int64_t resident = (int64_t)sm_count() * Few<BN>::CTAS;
-    LaunchConfig cfg(dim3((unsigned)few_ctas(g.M, g.N, g.K, resident < kFewMaxCtas ? resident : kFewMaxCtas)), Few<BN>::THREADS, smem, s);
+    static_assert(Few<BN>::CTAS == (BN <= 32 ? 2 : 1), "few_resident counts the same");
+    LaunchConfig cfg(dim3((unsigned)few_ctas(g.N, g.K, few_resident(g.M))), Few<BN>::THREADS, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
 }
 
@@ -766,34 +868,34 @@ cudaError_t launch_few(const Fp8Gemm& g, void* workspace, bool prepared, cudaStr
     p.M = (int)g.M;
     p.N = (int)g.N;
     p.blocks = (int)((g.K + 127) / 128);
-    p.tiles_a = few_tiles(g.M);
     p.bn = few_bn(g.M);
-    p.units = few_row_tiles(g.N) * p.tiles_a * p.blocks;
+    p.units = few_tiles(g.N) * p.blocks;
     p.arrived = static_cast<unsigned int*>(workspace);
-    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + few_arrived_bytes(g.M, g.N));
+    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + few_arrived_bytes(g.N));
     p.weights_ready = prepared;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
     if (!prepared) {
-        cudaError_t e = cudaMemsetAsync(workspace, 0, few_arrived_bytes(g.M, g.N), s);
+        cudaError_t e = cudaMemsetAsync(workspace, 0, few_arrived_bytes(g.N), s);
         if (e != cudaSuccess) return e;
     }
     switch (few_width(g.M)) {
         case 16: return launch_few_t<16, WT>(g, p, s);
         case 32: return launch_few_t<32, WT>(g, p, s);
-        case 64: return launch_few_t<64, WT>(g, p, s);
-        default: return launch_few_t<128, WT>(g, p, s);
+        default: return launch_few_t<64, WT>(g, p, s);
     }
 }
 
 }  // namespace
 
-size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return few_rows(M, N, K) ? few_arrived_bytes(M, N) + few_part_bytes(M, N, K) : 0;
+size_t fp8_gemm_zeroed_bytes(int64_t M, int64_t N, int64_t K) {
+    if (few_rows(M, N, K)) return few_arrived_bytes(N);
+    return pair_splits(M, N, K) > 1 ? pair_arrived_bytes(M, N) : 0;
 }
 
-size_t fp8_gemm_zeroed_bytes(int64_t M, int64_t N, int64_t K) {
-    return few_rows(M, N, K) ? few_arrived_bytes(M, N) : 0;
+size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (few_rows(M, N, K)) return few_arrived_bytes(N) + few_part_bytes(M, N, K);
+    return pair_splits(M, N, K) > 1 ? pair_arrived_bytes(M, N) + pair_part_bytes(M, N, K) : 0;
 }
 
 cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
@@ -811,7 +913,7 @@ cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cu
     }
     if (few_rows(g.M, g.N, g.K))
         return g.transpose ? launch_few<true>(g, workspace, prepared, s) : launch_few<false>(g, workspace, prepared, s);
-    return g.transpose ? launch_pair<true>(g, s) : launch_pair<false>(g, s);
+    return g.transpose ? launch_pair<true>(g, workspace, prepared, s) : launch_pair<false>(g, workspace, prepared, s);
 }
 
 }  // namespace wq
