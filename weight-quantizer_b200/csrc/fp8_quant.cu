@@ -18,36 +18,107 @@
 #include "launch.h"
 #include "tc_ptx.cuh"
 
+#include <type_traits>
+
 namespace wq {
 namespace {
 
-// Eight consecutive values of a row as fp32; `n` of them exist (the others
-// read as 0). VEC: the eight are 16-byte aligned in memory.
+// Eight consecutive values of a row, as they are in memory; `n` of them exist (the
+// others are 0). VEC: the eight are 16-byte aligned in memory.
+template <typename T>
+struct Eight {
+    static constexpr int WORDS = 8 * (int)sizeof(T) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t h = w[i >> 1];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value)   // a bf16 is the upper half of its fp32
+            return __uint_as_float(i & 1 ? h & 0xffff0000u : h << 16);
+        return __half2float(__ushort_as_half((unsigned short)(i & 1 ? h >> 16 : h & 0xffffu)));
+    }
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T* p, int n, Eight<T>& v) {
     if (VEC && n >= 8) {
-        constexpr int W = (int)(8 * sizeof(T) / 16);
-        uint4 r[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) r[i] = ld_stream_v4(reinterpret_cast<const uint4*>(p) + i);
-        const T* e = reinterpret_cast<const T*>(r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+        for (int i = 0; i < Eight<T>::WORDS / 4; ++i) {
+            const uint4 r = ld_stream_v4(reinterpret_cast<const uint4*>(p) + i);
+            v.w[4 * i] = r.x, v.w[4 * i + 1] = r.y, v.w[4 * i + 2] = r.z, v.w[4 * i + 3] = r.w;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(p[i]) : 0.0f;
+        for (int i = 0; i < Eight<T>::WORDS; ++i) v.w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i < n) {
+                if constexpr (sizeof(T) == 4) v.w[i] = __float_as_uint(to_f32<T>(p[i]));
+                else v.w[i >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
+            }
+        }
     }
 }
 
-// Codes of eight values; `n` of them are written. VEC: 8-byte aligned.
-__device__ __forceinline__ void store8(uint8_t* p, int n, const float (&v)[8], float inv, bool vec) {
-    uint2 w;
-    w.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
-    w.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
-    if (vec && n >= 8) {
-        *reinterpret_cast<uint2*>(p) = w;
+// The largest magnitude of a block, held as its bits, which order magnitudes as
+// whole numbers (two 16-bit values in a word, or one fp32): no conversions, and a
+// value that is not finite shows as bits of at least the infinity's.
+template <typename T>
+struct Top {
+    static constexpr bool WIDE = sizeof(T) == 4;
+    static constexpr uint32_t INF =
+        WIDE ? 0x7f800000u : (std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u);
+    static __device__ __forceinline__ uint32_t of(uint32_t w) { return w & (WIDE ? 0x7fffffffu : 0x7fff7fffu); }
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        return WIDE ? (a > b ? a : b) : __vmaxu2(a, b);
+    }
+    // each magnitude that is not finite replaced by 0
+    static __device__ __forceinline__ uint32_t finite(uint32_t a) {
+        return WIDE ? (a >= INF ? 0u : a) : a & __vcmpltu2(a, INF);
+    }
+    static __device__ __forceinline__ bool all_finite(uint32_t a) {
+        return WIDE ? a < INF : __vcmpltu2(a, INF) == 0xffffffffu;
+    }
+    static __device__ __forceinline__ float value(uint32_t a) {   // the larger half's
+        if constexpr (WIDE) return __uint_as_float(a);
+        const uint32_t h = (a >> 16) > (a & 0xffffu) ? a >> 16 : a & 0xffffu;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(h << 16);
+        return __half2float(__ushort_as_half((unsigned short)h));
+    }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t top8(const Eight<T>& v) {
+    uint32_t m = Top<T>::of(v.w[0]);
+#pragma unroll
+    for (int i = 1; i < Eight<T>::WORDS; ++i) m = Top<T>::max(m, Top<T>::of(v.w[i]));
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top8_finite(const Eight<T>& v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < Eight<T>::WORDS; ++i) m = Top<T>::max(m, Top<T>::finite(Top<T>::of(v.w[i])));
+    return m;
+}
+
+// Codes of eight values; `n` of them are written. vec: 8-byte aligned. all_finite:
+// no NaN or infinity is among them, which saves the test of each.
+template <typename T>
+__device__ __forceinline__ void store8(uint8_t* p, int n, const Eight<T>& v, float inv, bool vec, bool all_finite) {
+    uint32_t w[2];
+    if (all_finite) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = e4m3x2_finite(v.at(4 * i) * inv, v.at(4 * i + 1) * inv) |
+                   (e4m3x2_finite(v.at(4 * i + 2) * inv, v.at(4 * i + 3) * inv) << 16);
     } else {
-        const uint64_t u = (uint64_t)w.x | ((uint64_t)w.y << 32);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = e4m3x2(v.at(4 * i) * inv, v.at(4 * i + 1) * inv) |
+                   (e4m3x2(v.at(4 * i + 2) * inv, v.at(4 * i + 3) * inv) << 16);
+    }
+    if (vec && n >= 8) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+        const uint64_t u = (uint64_t)w[0] | ((uint64_t)w[1] << 32);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < n) p[i] = (uint8_t)(u >> (8 * i));
@@ -76,7 +147,7 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, 
     const int64_t nb = (cols + kFp8Block - 1) / kFp8Block;
     const int64_t j0 = (int64_t)blockIdx.y * kBlocksPerThread;
     const bool live = row < rows;
-    float v[kBlocksPerThread][8];
+    Eight<T> v[kBlocksPerThread];
 #pragma unroll
     for (int i = 0; i < kBlocksPerThread; ++i) {
         const int64_t c = (j0 + i) * kFp8Block + sub * 8;
@@ -85,16 +156,16 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, 
     }
 #pragma unroll
     for (int i = 0; i < kBlocksPerThread; ++i) {
-        float m = 0.0f;
+        uint32_t m = top8(v[i]);
+        const bool fine = __all_sync(0xffffffffu, Top<T>::all_finite(m));
+        if (!fine) m = top8_finite(v[i]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int e = fp8_scale_exponent(m);
+        for (int o = 8; o > 0; o >>= 1) m = Top<T>::max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e = fp8_scale_exponent(Top<T>::value(m));
         const int64_t j = j0 + i;
         const int64_t c = j * kFp8Block + sub * 8;
         const int64_t left = live ? cols - c : 0;
-        if (left > 0) store8(codes + row * ldc + c, left >= 8 ? 8 : (int)left, v[i], pow2i(-e), vec_out);
+        if (left > 0) store8(codes + row * ldc + c, left >= 8 ? 8 : (int)left, v[i], pow2i(-e), vec_out, fine);
         if (live && j < nb && sub == 0) scales[row * s_row + j * s_col] = pow2i(e);
     }
 }
@@ -106,34 +177,40 @@ __global__ void __launch_bounds__(256) fp8_tiles_kernel(const T* __restrict__ x,
                                                         int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc,
                                                         bool vec_out, float* __restrict__ scales, int64_t s_row,
                                                         int64_t s_col, int64_t nb) {
-    __shared__ float red[8];
+    __shared__ uint32_t red[8];
     const int64_t bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;
     const int sub = threadIdx.x & 15;
     const int64_t r0 = bi * kFp8Block + (threadIdx.x >> 4);
     const int64_t c = bj * kFp8Block + sub * 8;
     const int64_t left = cols - c;
     const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    float v[8][8];
-    float m = 0.0f;
+    Eight<T> v[8];
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = r0 + 16 * i;
         load8<T, VEC>(x + r * ldx + c, r < rows ? n : 0, v[i]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < 8; ++i) m = Top<T>::max(m, top8(v[i]));
+    const bool fine = __syncthreads_and(Top<T>::all_finite(m)) != 0;
+    if (!fine) {
+        m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = Top<T>::max(m, top8_finite(v[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = Top<T>::max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
-    const int e = fp8_scale_exponent(m);
+    for (int w = 0; w < 8; ++w) m = Top<T>::max(m, red[w]);
+    const int e = fp8_scale_exponent(Top<T>::value(m));
     const float inv = pow2i(-e);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = r0 + 16 * i;
-        if (r < rows && n > 0) store8(codes + r * ldc + c, n, v[i], inv, vec_out);
+        if (r < rows && n > 0) store8(codes + r * ldc + c, n, v[i], inv, vec_out, fine);
     }
     if (threadIdx.x == 0) scales[bi * s_row + bj * s_col] = pow2i(e);
 }
@@ -169,10 +246,10 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x
     float acc[8] = {};
 #pragma unroll 4
     for (int64_t r = lane; r < rows; r += 32) {
-        float v[8];
+        Eight<T> v;
         load8<T, VEC>(x + r * ldx + c, n, v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+        for (int k = 0; k < 8; ++k) acc[k] += v.at(k);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) part[lane][sub * 8 + k] = acc[k];

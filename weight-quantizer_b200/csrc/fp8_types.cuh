@@ -40,10 +40,13 @@ __device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
 // Two e4m3 codes (a in the low byte): nearest, ties to even. Codes have no
 // infinity: an input that is not finite becomes the NaN code, so that an
 // overflow upstream stays visible instead of reading as 448.
+__device__ __forceinline__ uint32_t e4m3x2_finite(float a, float b) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
     a = fabsf(a) <= 3.402823466e38f ? a : __int_as_float(0x7fc00000);
     b = fabsf(b) <= 3.402823466e38f ? b : __int_as_float(0x7fc00000);
-    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    return e4m3x2_finite(a, b);
 }
 
 // The values of two codes; every e4m3 value is exact in fp16.
@@ -64,12 +67,6 @@ __device__ __forceinline__ int fp8_scale_exponent(float amax) {
     const int e = (int)(u >> 23) - 127;
     const int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
     return k < -117 ? -117 : k;
-}
-
-// |v| for the block's maximum: values that are not finite do not take part.
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a <= 3.402823466e38f ? a : 0.0f;
 }
 
 }  // namespace wq
