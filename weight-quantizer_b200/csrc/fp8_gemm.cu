@@ -11,6 +11,8 @@
 
 #include "launch.h"
 
+#include <type_traits>
+
 namespace wq {
 namespace {
 
@@ -34,6 +36,9 @@ namespace {
 
 constexpr int kPairTile = 256;
 constexpr int kPairStages = 6;                      // even: each issuing warp has its own
+constexpr int kPairScaleSlots = 3;                  // blocks whose scales are on their way
+constexpr int kPairScaleBytes = (128 + 4) * 4;      // a's of the CTA's rows, w's of its two column blocks
+constexpr int kOutBytes = 4096;                     // a summing warp's part of y on its way out
 constexpr int kOperandBytes = 128 * 128;            // one operand of one CTA for one block
 constexpr int kPairStage = 2 * kOperandBytes;
 constexpr int kPairThreads = 384;
@@ -41,10 +46,13 @@ constexpr int kPairLaunchRegs = 168, kPairCtlRegs = 56, kPairSumRegs = 224;
 static_assert(kPairCtlRegs + 2 * kPairSumRegs <= 3 * kPairLaunchRegs, "register split exceeds the launch's registers");
 
 struct PairSmem {
-    static constexpr int BAR = kPairStages * kPairStage;
+    static constexpr int OUT = kPairStages * kPairStage;
+    static constexpr int SCALES = OUT + 8 * kOutBytes;
+    static constexpr int BAR = SCALES + kPairScaleSlots * kPairScaleBytes;
     // full and done per stage (done: the block's MMAs are over, so its operands
     // may be replaced and its sums read); sums empty[2]
-    static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 2);
+    // per scale slot there, read
+    static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 2 + 2 * kPairScaleSlots);
     static constexpr int FLAG = TMEM_SLOT + 8;
     static constexpr int TOTAL = TMEM_SLOT + 16;
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
@@ -58,11 +66,10 @@ struct PairParams {
     const void* bias;
     int bias_type;
     void* out;
-    int out_type;
     int64_t ldo;
     int M, N, blocks;        // inner blocks of 128
     int tiles_m, tiles_n, band;
-    bool wide_out;           // rows of out are 32-byte aligned
+    bool tma_out;            // rows of out are 16-byte aligned
     int splits;              // parts of the inner blocks, each a tile's work for a pair of its own
     float* part;             // [tile][split][rank] sums of 128 x 256
     unsigned int* arrived;   // [tile][rank], zeroed before the launch
@@ -79,43 +86,59 @@ __device__ __forceinline__ void tile_of(int t, const PairParams& p, int& mt, int
     mt = b * p.band + (in - nt * bw);
 }
 
-// 32 columns (c .. c + 31) of row m of y from fp32 sums.
+// A warp's 32 rows (from m0) x 128 columns (from n0) of y out of its sums: a lane is
+// a row. By way of shared memory (128 bytes of 32 rows at a time, swizzled) and a TMA
+// store that ends at y's edges and drains while the next tile's blocks are summed:
+// stores from registers held the tile's hand-off for 4300 cycles, every CTA's 64 KB
+// at once.
 template <typename O>
-__device__ __forceinline__ void store32(O* row, int64_t c, int64_t n, bool wide, const float (&v)[32], const void* bias,
-                                        int bias_type) {
-    float b[32];
-    if (bias != nullptr) {
+__device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap* map, uint32_t out, int lane,
+                                         int64_t m0, int64_t n0, const uint64_t (&acc)[64]) {
+    constexpr int PER = 16 / (int)sizeof(O);      // values in 16 bytes
+    constexpr int BOX = 8 * PER;                  // columns in 128 bytes
+    const bool has_bias = p.bias != nullptr;
+    auto value = [&](int c) {
+        const float2 f = unpack2(acc[c / 2]);
+        float v = c & 1 ? f.y : f.x;
+        if (has_bias && n0 + c < p.N) v += load_any(p.bias, p.bias_type, n0 + c);
+        return from_f32<O>(v);
+    };
+    if (p.tma_out) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) b[i] = c + i < n ? load_any(bias, bias_type, c + i) : 0.0f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) b[i] = -0.0f;   // leaves every value as it is
-    }
-    if (wide && c + 32 <= n) {
-        constexpr int PER = 4 / (int)sizeof(O);       // values in a word
-#pragma unroll
-        for (int i = 0; i < 32; i += 8 * PER) {
-            uint32_t w[8];
+        for (int c0 = 0; c0 < 128; c0 += BOX) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
+                uint32_t w[4];
                 O e[PER];
 #pragma unroll
-                for (int j = 0; j < PER; ++j) e[j] = from_f32<O>(v[i + k * PER + j] + b[i + k * PER + j]);
-                w[k] = *reinterpret_cast<const uint32_t*>(e);
-            }
-            st_32(row + c + i, w);
-        }
-    } else {
+                for (int j = 0; j < PER; ++j) e[j] = value(c0 + k * PER + j);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (c + i < n) row[c + i] = from_f32<O>(v[i] + b[i]);
+                for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint32_t*>(e)[j];
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((k ^ (lane & 7)) << 4)),
+                             "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                             : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (m0 < p.M && n0 + c0 < p.N) tma_store(map, (int)(n0 + c0), (int)m0, out);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        }
+    } else if (m0 + lane < p.M) {
+        O* row = static_cast<O*>(p.out) + (m0 + lane) * p.ldo + n0;
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+            if (n0 + c < p.N) row[c] = value(c);
     }
 }
 
-template <bool WT, bool SPLIT>
+template <bool WT, bool SPLIT, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     fp8_gemm_pair_kernel(const PairParams p, const __grid_constant__ CUtensorMap map_a,
-                         const __grid_constant__ CUtensorMap map_w) {
+                         const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y) {
     using L = PairSmem;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem =
@@ -127,6 +150,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     auto full = [&](int s) { return bar(s); };
     auto done = [&](int s) { return bar(kPairStages + s); };
     auto sums_empty = [&](int b) { return bar(2 * kPairStages + b); };
+    auto scaled = [&](int c) { return bar(2 * kPairStages + 2 + c); };
+    auto scales_read = [&](int c) { return bar(2 * kPairStages + 2 + kPairScaleSlots + c); };
     launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
@@ -135,6 +160,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         for (int b = 0; b < 2; ++b)
             mbar_init(sums_empty(b), 16);   // the even CTA's: one arrival per summing warp of the pair
+        for (int c = 0; c < kPairScaleSlots; ++c) {
+            mbar_init(scaled(c), 32);
+            mbar_init(scales_read(c), 8);
+        }
         fence_mbarrier_init();
     }
     if (warp == 1) tmem_alloc<2>(sbase + L::TMEM_SLOT, 512);
@@ -229,6 +258,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     ph ^= 1u;
                 }
             }
+        } else if (warp == 3) {
+            // each block's scales, by asynchronous copies (loaded into registers by the
+            // summing warps they were waited for: three blocks ahead was too late for
+            // scales that come from memory, and more cost registers)
+            int c = 0;
+            uint32_t ph = 1;
+            for (int t = first; t < items; t += pairs) {
+                int mt, nt;
+                tile_of(t / splits, p, mt, nt);
+                const int64_t m0 = (int64_t)mt * kPairTile + rank * 128 + lane;
+                const int b0 = from_block(t), b1 = to_block(t);
+                const float* sa = p.sa + m0 * p.sa_row + b0 * p.sa_col;
+                const float* sw = p.sw + min(2 * nt + (lane & 1), (p.N - 1) >> 7) * p.sw_n + b0 * p.sw_k;
+                for (int b = b0; b < b1; ++b) {
+                    if (!faulted && !mbar_wait_bounded(scales_read(c), ph)) give_up();
+                    __syncwarp();
+                    const uint32_t to = sbase + (uint32_t)(L::SCALES + c * kPairScaleBytes);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool some = m0 + 32 * j < p.M;   // rows beyond the last: 0
+                        cp_async4_s(to + (32 * j + lane) * 4, some ? sa + 32 * j * p.sa_row : p.sa, some);
+                    }
+                    if (lane < 2) cp_async4_s(to + (128 + lane) * 4, sw, true);
+                    cp_async_arrive(scaled(c));
+                    sa += p.sa_col;
+                    sw += p.sw_k;
+                    if (++c == kPairScaleSlots) {
+                        c = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairSumRegs));
@@ -238,45 +300,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         int64_t i = 0;
         int s = 0;
         uint32_t ph = 0;
+        int c = 0;
+        uint32_t cph = 0;
         for (int t = first; t < items; t += pairs) {
             int mt, nt;
             tile_of(t / splits, p, mt, nt);
             const int b0 = from_block(t), b1 = to_block(t);
-            const int64_t m = (int64_t)mt * kPairTile + rank * 128 + q * 32 + lane;
-            const int64_t n0 = (int64_t)nt * kPairTile + half * 128;
-            const float* sa = p.sa + min(m, (int64_t)p.M - 1) * p.sa_row;
-            const float* sw = p.sw + min(n0, (int64_t)p.N - 1) / 128 * p.sw_n;
             uint64_t acc[64];
 #pragma unroll
             for (int c = 0; c < 64; ++c) acc[c] = 0;
-            // the scales of the next three blocks are on their way
-            sa += b0 * p.sa_col, sw += b0 * p.sw_k;
-            float a1 = __ldg(sa), w1 = __ldg(sw), a2 = 0, w2 = 0, a3 = 0, w3 = 0;
-            if (b0 + 1 < b1) a2 = __ldg(sa + p.sa_col), w2 = __ldg(sw + p.sw_k);
-            if (b0 + 2 < b1) a3 = __ldg(sa + 2 * p.sa_col), w3 = __ldg(sw + 2 * p.sw_k);
-            for (int b = 0; b < b1 - b0; ++b, ++i) {
+            for (int b = b0; b < b1; ++b, ++i) {
                 const int buf = (int)(i & 1);
-                const float sc = a1 * w1;
-                a1 = a2, w1 = w2, a2 = a3, w2 = w3;
-                if (b + 3 < b1 - b0) a3 = __ldg(sa + (b + 3) * p.sa_col), w3 = __ldg(sw + (b + 3) * p.sw_k);
-                const uint64_t sc2 = pack2(sc, sc);
                 const uint32_t from = taddr + (uint32_t)(buf * 256);
                 uint64_t v[32];
-                if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
+                if (!try_wait_both(done(s), ph, scaled(c), cph)) {
+                    if (!faulted && !mbar_wait_bounded(scaled(c), cph)) give_up();
+                    if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
+                }
                 __syncwarp();
                 tc_after();
+                const float* scales = reinterpret_cast<const float*>(smem + L::SCALES + c * kPairScaleBytes);
+                const float sc = scales[q * 32 + lane] * scales[128 + half];
+                const uint64_t sc2 = pack2(sc, sc);
                 tmem_pairs(from, v);
 #pragma unroll
                 for (int c = 0; c < 32; ++c) fma2(acc[c], v[c], sc2);
                 tmem_pairs(from + 64u, v);
                 tc_before();
                 __syncwarp();
-                if (lane == 0) arrive_in_cluster(free0 + 8u * (uint32_t)buf);
+                if (lane == 0) {
+                    arrive_in_cluster(free0 + 8u * (uint32_t)buf);
+                    mbar_arrive(scales_read(c));
+                }
 #pragma unroll
-                for (int c = 0; c < 32; ++c) fma2(acc[32 + c], v[c], sc2);
+                for (int k = 0; k < 32; ++k) fma2(acc[32 + k], v[k], sc2);
                 if (++s == kPairStages) {
                     s = 0;
                     ph ^= 1u;
+                }
+                if (++c == kPairScaleSlots) {
+                    c = 0;
+                    cph ^= 1u;
                 }
             }
             bool write = true;
@@ -318,27 +382,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     }
                 }
             }
-            if (write && m < p.M) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float v[32];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 f = unpack2(acc[16 * c + k]);
-                        v[2 * k] = f.x;
-                        v[2 * k + 1] = f.y;
-                    }
-                    const int64_t col = n0 + 32 * c;
-                    if (p.out_type == kBf16)
-                        store32(static_cast<__nv_bfloat16*>(p.out) + m * p.ldo, col, p.N, p.wide_out, v, p.bias,
-                                p.bias_type);
-                    else if (p.out_type == kF16)
-                        store32(static_cast<__half*>(p.out) + m * p.ldo, col, p.N, p.wide_out, v, p.bias, p.bias_type);
-                    else
-                        store32(static_cast<float*>(p.out) + m * p.ldo, col, p.N, p.wide_out, v, p.bias, p.bias_type);
-                }
-            }
+            if (write)
+                put_tile<O>(p, &map_y, sbase + (uint32_t)(L::OUT + (warp - 4) * kOutBytes), lane,
+                            (int64_t)mt * kPairTile + rank * 128 + q * 32, (int64_t)nt * kPairTile + half * 128, acc);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     tc_before();
     __syncthreads();
@@ -691,8 +739,6 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
 
 // ---- host side ------------------------------------------------------------------------
 
-int type_bytes(int t) { return t == kF32 ? 4 : 2; }
-
 // y = bias, or 0, in every row: a product without inner values.
 template <typename O>
 __global__ void fill_rows_kernel(O* out, int64_t M, int64_t N, int64_t ldo, const void* bias, int bias_type) {
@@ -724,8 +770,8 @@ size_t pair_part_bytes(int64_t M, int64_t N, int64_t K) {
     return (size_t)pair_tiles(M, N) * pair_splits(M, N, K) * 2 * 128 * 256 * 4;
 }
 
-template <bool WT, bool SPLIT>
-cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
+template <bool WT, bool SPLIT, typename O>
+cudaError_t launch_pair_o(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
     PairParams p;
     p.sa = g.a.scales;
     p.sa_row = g.a.s_row;
@@ -736,7 +782,6 @@ cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     p.bias = g.bias;
     p.bias_type = g.bias_type;
     p.out = g.out;
-    p.out_type = g.out_type;
     p.ldo = g.ldo;
     p.M = (int)g.M;
     p.N = (int)g.N;
@@ -749,19 +794,24 @@ cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     band = band < 1 ? 1 : band;
     const int64_t bands = (p.tiles_m + band - 1) / band;
     p.band = (int)((p.tiles_m + bands - 1) / bands);
-    p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * type_bytes(g.out_type)) % 32 == 0;
     p.splits = splits;
     p.arrived = static_cast<unsigned int*>(workspace);
     p.part = SPLIT ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pair_arrived_bytes(g.M, g.N))
                    : nullptr;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
-    CUtensorMap ma, mw;
+    CUtensorMap ma, mw, my = {};
     if (!encode_codes(&ma, g.a.codes, g.a.cols, g.a.rows, g.a.ld, 128) ||
         !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, 128))
         return cudaErrorInvalidValue;
+    constexpr CUtensorMapDataType DT = sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : std::is_same<O, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int64_t out_pitch = g.M > 1 ? g.ldo * (int64_t)sizeof(O) : (g.N * (int64_t)sizeof(O) + 15) / 16 * 16;
+    p.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && out_pitch % 16 == 0 &&
+                encode_rows(&my, DT, (int)sizeof(O), g.out, g.N, g.M, out_pitch, 32);
     const size_t smem = (size_t)PairSmem::TOTAL + 1024;
-    auto kern = fp8_gemm_pair_kernel<WT, SPLIT>;
+    auto kern = fp8_gemm_pair_kernel<WT, SPLIT, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kPairLaunchRegs, ready);
     if (e != cudaSuccess) return e;
@@ -769,7 +819,14 @@ cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     const int64_t pairs = sm_count() / 2;
     if (items > 0x7fffffff) return cudaErrorInvalidValue;
     LaunchConfig cfg(dim3(2u * (unsigned)(items < pairs ? items : pairs)), kPairThreads, smem, s);
-    return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw);
+    return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw, my);
+}
+
+template <bool WT, bool SPLIT>
+cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
+    if (g.out_type == kF16) return launch_pair_o<WT, SPLIT, __half>(g, splits, workspace, s);
+    if (g.out_type == kBf16) return launch_pair_o<WT, SPLIT, __nv_bfloat16>(g, splits, workspace, s);
+    return launch_pair_o<WT, SPLIT, float>(g, splits, workspace, s);
 }
 
 template <bool WT>

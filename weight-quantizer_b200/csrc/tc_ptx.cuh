@@ -274,6 +274,14 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             : "memory");
 }
 
+// TMA box store from this CTA's shared memory (in this thread's current bulk group).
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+
 // Arrives on `bar` when this thread's asynchronous copies so far are done (one of
 // the arrivals that the barrier was set up for).
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
