@@ -8,9 +8,11 @@
 // for fp16, three for fp32): every product is exact. Other scales' code * scale is
 // rounded to bf16 (half a step 2^-9 of each value), the operand type's only choice.
 //
-// Sums over 512 rows stay in tensor memory, then they are added to fp32 registers:
-// the tensor core's own additions cut off what they add, and over all rows of a
-// long batch that would grow to several steps of the result, all to one side.
+// Sums over 512 rows (256 and 128 with two and three terms) stay in tensor memory,
+// then they are added to fp32 registers: the tensor core's own additions cut off what
+// they add, and over all rows of a long batch that grows, all to one side. Relative
+// error at 8192 rows of random signs 3.6e-6 without the spans and 1.6e-7 with them
+// (1.3e-5 and 3.4e-7 where every product is positive).
 #include "fp8_types.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -33,7 +35,6 @@ namespace {
 
 constexpr int kTile = 256;
 constexpr int kStep = 64;                      // rows of dy and x per step
-constexpr int kSpan = 8;                       // steps whose sums stay in tensor memory
 constexpr int kPlaneBytes = kStep * 128 * 2;   // 64 rows x 128 columns in bf16: one CTA's operand of one step
 constexpr int kThreads = 640;
 constexpr int kLaunchRegs = 96, kCtlRegs = 40, kMakeRegs = 56, kSumRegs = 160;
@@ -46,6 +47,8 @@ constexpr int kCodesBytes = kStep * 128;
 // P terms of dy per step, then x^; the codes on their way, their scales.
 template <int P>
 struct Smem {
+    // steps whose sums stay in tensor memory: some 32 MMAs whatever the terms
+    static constexpr int SPAN = P == 1 ? 8 : (P == 2 ? 4 : 2);
     static constexpr int STAGE = (P + 1) * kPlaneBytes;
     static constexpr int STAGES = (222 * 1024 - kAhead * (kCodesBytes + kStep * 4)) / STAGE;
     static constexpr int CODES = STAGES * STAGE;
@@ -213,12 +216,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t ph = 0, reuse = 1;
             for (int t = 0; t < mine; ++t) {
                 for (int i = 0; i < p.steps; ++i) {
-                    const int in = i % kSpan;
+                    const int in = i % L::SPAN;
                     if (in == 0) wait(sums_empty(buf), reuse);
                     wait(full(s), ph);
                     __syncwarp();
                     tc_after();
-                    const bool last = in == kSpan - 1 || i == p.steps - 1;
+                    const bool last = in == L::SPAN - 1 || i == p.steps - 1;
                     if (elect_one()) {
                         const uint64_t d0 = desc0 + (uint64_t)(s * (L::STAGE >> 4));
                         const uint64_t dx = d0 + (uint64_t)(P * (kPlaneBytes >> 4));
@@ -373,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             float acc[128];
 #pragma unroll
             for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
-            for (int i = 0; i < p.steps; i += kSpan) {
+            for (int i = 0; i < p.steps; i += L::SPAN) {
                 wait(sums_full(buf), ph);
                 __syncwarp();
                 tc_after();
