@@ -754,9 +754,14 @@ def _codes_arg(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
         plain = codes.view(torch.uint8)
     else:
         plain = codes.contiguous().view(torch.uint8)
-    kept = torch.empty((rows, pitch), dtype=torch.uint8, device=codes.device)
+    kept = _empty(rows, pitch, torch.uint8, codes.device)
     kept[:, :cols].copy_(plain)
     return kept, pitch
+
+
+def _empty(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """A dense matrix (torch.empty takes half again as long as the strided form)."""
+    return torch.empty_strided((rows, cols), (cols if cols > 0 else 1, 1), dtype=dtype, device=dev)
 
 
 def fp8_quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -767,13 +772,13 @@ def fp8_quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.
     rows, cols = x.shape
     pitch = (cols + 15) // 16 * 16
     nb = (cols + FP8_BLOCK - 1) // FP8_BLOCK
-    codes = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=dev)
+    codes = _empty(rows, pitch, torch.float8_e4m3fn, dev)
     if block_rows == 1:
         s_row, s_col = 1, max(rows, 1)   # one block's scales of all rows side by side
         scales = torch.empty_strided((rows, nb), (1, s_col), dtype=torch.float32, device=dev)
     else:
         s_row, s_col = max(nb, 1), 1
-        scales = torch.empty(((rows + FP8_BLOCK - 1) // FP8_BLOCK, nb), dtype=torch.float32, device=dev)
+        scales = _empty((rows + FP8_BLOCK - 1) // FP8_BLOCK, nb, torch.float32, dev)
     _fp8_call(library().wq_fp8_quantize, dev,
               (x.data_ptr(), x_type, rows, cols, ldx, block_rows, codes.data_ptr(), pitch, scales.data_ptr(), s_row,
                s_col))
@@ -786,7 +791,7 @@ def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, block_rows: int, d
     dev = _fp8_device(codes, scales)
     codes, ld = _rows(codes)
     rows, cols = codes.shape
-    out = torch.empty((rows, cols), dtype=dtype, device=dev)
+    out = _empty(rows, cols, dtype, dev)
     _fp8_call(library().wq_fp8_dequantize, dev,
               (codes.data_ptr(), rows, cols, ld, block_rows, scales.data_ptr(), *scales.stride(), out.data_ptr(),
                out_type, max(cols, 1)))
@@ -796,7 +801,7 @@ def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, block_rows: int, d
 def _out_arg(out: torch.Tensor | None, rows: int, cols: int, dtype: torch.dtype,
              dev: torch.device) -> tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty((rows, cols), dtype=dtype, device=dev), max(cols, 1)
+        return _empty(rows, cols, dtype, dev), max(cols, 1)
     if out.dtype != dtype or out.device != dev or tuple(out.shape) != (rows, cols):
         raise ValueError(f"out must be a {dtype} [{rows}, {cols}] tensor on the inputs' device")
     if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
@@ -834,7 +839,7 @@ def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor | None, w: torch.Tensor, w_
     ws_ptr = None
     nws = (lib.wq_fp8_linear_workspace_bytes if a_scales is None else lib.wq_fp8_gemm_workspace_bytes)(M, N, K)
     if nws:
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev)
         ws_ptr = ws.data_ptr()
     if a_scales is None:
         x_type = _dtype(a.dtype, "a")
@@ -862,7 +867,7 @@ def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     codes, ld = _codes_arg(codes)
     lib = library()
     nws = lib.wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev) if nws else None
     _fp8_call(lib.wq_fp8_weight_grad, dev,
               (dy.data_ptr(), dy_type, M, N, ldy, codes.data_ptr(), K, ld, scales.data_ptr(), *scales.stride(),
                dw.data_ptr(), out_type, ldw, int(accumulate), None if ws is None else ws.data_ptr(), nws), True)

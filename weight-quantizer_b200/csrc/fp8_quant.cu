@@ -232,32 +232,40 @@ __global__ void __launch_bounds__(256) fp8_values_kernel(const uint8_t* __restri
     }
 }
 
-// out[n] = sum_m x[m, n] in fp32: a CTA takes 64 columns, 8 threads side by
-// side (8 columns each) times 32 row lanes; each thread adds its rows in
-// order, then the lanes are added in order (the same bits on every call).
+// out[n] = sum_m x[m, n] in fp32: a CTA takes 64 columns, 8 threads side by side
+// (8 columns each) times 64 row lanes; each thread adds its rows in order, then the
+// lanes are added in order (the same bits on every call). There are few CTAs, so each
+// thread has eight loads in flight.
+constexpr int kSumLanes = 64;
 template <typename T, typename O, bool VEC>
-__global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
-                                                         int64_t ldx, O* __restrict__ out) {
-    __shared__ float part[32][65];
+__global__ void __launch_bounds__(8 * kSumLanes) column_sum_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                                   int64_t ldx, O* __restrict__ out) {
+    __shared__ float part[kSumLanes][65];
     const int sub = threadIdx.x & 7, lane = threadIdx.x >> 3;
     const int64_t c = (int64_t)blockIdx.x * 64 + sub * 8;
     const int64_t left = cols - c;
     const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
     float acc[8] = {};
-#pragma unroll 4
-    for (int64_t r = lane; r < rows; r += 32) {
-        Eight<T> v;
-        load8<T, VEC>(x + r * ldx + c, n, v);
+    constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;
+    for (int64_t r = lane; r < rows; r += AHEAD * kSumLanes) {
+        Eight<T> v[AHEAD];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v.at(k);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int64_t at = r + i * kSumLanes;
+            load8<T, VEC>(x + at * ldx + c, at < rows ? n : 0, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += v[i].at(k);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) part[lane][sub * 8 + k] = acc[k];
     __syncthreads();
     if (threadIdx.x < 64 && (int64_t)blockIdx.x * 64 + threadIdx.x < cols) {
         float s = 0.0f;
-#pragma unroll
-        for (int l = 0; l < 32; ++l) s += part[l][threadIdx.x];
+#pragma unroll 16
+        for (int l = 0; l < kSumLanes; ++l) s += part[l][threadIdx.x];
         out[(int64_t)blockIdx.x * 64 + threadIdx.x] = from_f32<O>(s);
     }
 }
@@ -301,9 +309,9 @@ cudaError_t column_sum_t(const T* x, int64_t rows, int64_t cols, int64_t ldx, O*
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
     const unsigned grid = (unsigned)((cols + 63) / 64);
     if (vec)
-        column_sum_kernel<T, O, true><<<grid, 256, 0, s>>>(x, rows, cols, ldx, out);
+        column_sum_kernel<T, O, true><<<grid, 8 * kSumLanes, 0, s>>>(x, rows, cols, ldx, out);
     else
-        column_sum_kernel<T, O, false><<<grid, 256, 0, s>>>(x, rows, cols, ldx, out);
+        column_sum_kernel<T, O, false><<<grid, 8 * kSumLanes, 0, s>>>(x, rows, cols, ldx, out);
     return cudaGetLastError();
 }
 
