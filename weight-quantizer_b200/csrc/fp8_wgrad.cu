@@ -21,7 +21,7 @@
 namespace wq {
 namespace {
 
-// A pair of CTAs makes a 256 x 256 tile of dw with tcgen05.mma of cta_group::2 on
+// A pair of CTAs makes a 256 x TK tile of dw with tcgen05.mma of cta_group::2 on
 // steps of 64 rows of dy and x. Both operands lie along the outer dimension in
 // memory (MN-major), so dy goes from memory to the MMA as it is: warp 0 loads
 // boxes of 64 rows x 64 columns. x^ is made by eight warps (4-11), which take turns
@@ -31,11 +31,13 @@ namespace {
 // takes eight codes of each 64 columns, which are one 16-byte chunk of that tile, so
 // that eight lanes fill a row without bank conflicts. Eight more warps
 // (12-19) add the finished sums of 512 rows to their registers: a lane is a row of
-// dw, a warp has 128 columns.
+// dw, a warp has TK / 2 columns. TK is 256, or 128 where that fills the SMs better
+// (a step of the narrow tile takes a little over half as long; 2304 x 768 is 27 wide
+// tiles for 74 pairs, or 54 narrow ones).
 
-constexpr int kTile = 256;
+constexpr int kRows = 256;                     // rows of dw in a tile
 constexpr int kStep = 64;                      // rows of dy and x per step
-constexpr int kPlaneBytes = kStep * 128 * 2;   // 64 rows x 128 columns in bf16: one CTA's operand of one step
+constexpr int kPlaneBytes = kStep * 128 * 2;   // 64 rows x 128 columns in bf16: one CTA's term of dy in one step
 constexpr int kThreads = 640;
 constexpr int kLaunchRegs = 96, kCtlRegs = 40, kMakeRegs = 56, kSumRegs = 160;
 static_assert(kCtlRegs + 2 * kMakeRegs + 2 * kSumRegs <= 5 * kLaunchRegs, "register split exceeds the launch's registers");
@@ -45,11 +47,12 @@ constexpr int kAhead = 6;
 constexpr int kCodesBytes = kStep * 128;
 
 // P terms of dy per step, then x^; the codes on their way, their scales.
-template <int P>
+template <int P, int TK>
 struct Smem {
     // steps whose sums stay in tensor memory: some 32 MMAs whatever the terms
     static constexpr int SPAN = P == 1 ? 8 : (P == 2 ? 4 : 2);
-    static constexpr int STAGE = (P + 1) * kPlaneBytes;
+    static constexpr int X_BYTES = kStep * (TK / 2) * 2;
+    static constexpr int STAGE = P * kPlaneBytes + X_BYTES;
     static constexpr int STAGES = (222 * 1024 - kAhead * (kCodesBytes + kStep * 4)) / STAGE;
     static constexpr int CODES = STAGES * STAGE;
     static constexpr int SCALES = CODES + kAhead * kCodesBytes;
@@ -110,11 +113,11 @@ __device__ __forceinline__ void put16(O* row, int64_t c, int64_t k, bool wide, c
     }
 }
 
-template <int P, typename O>
+template <int P, int TK, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy,
                      const __grid_constant__ CUtensorMap map_x) {
-    using L = Smem<P>;
+    using L = Smem<P, TK>;
     constexpr int NS = L::STAGES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem =
@@ -176,7 +179,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int t = first; t < tiles; t += pairs) {
                 int nt, kt;
                 tile_of(t, p, nt, kt);
-                const int n0 = nt * kTile + rank * 128;
+                const int n0 = nt * kRows + rank * 128;
                 for (int i = 0; i < p.steps; ++i) {
                     wait(done(s), ph);
                     __syncwarp();
@@ -210,7 +213,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp == 1 && rank == 0) {
-            constexpr uint32_t idesc = mma_idesc(1, true, true, kTile, kTile);
+            constexpr uint32_t idesc = mma_idesc(1, true, true, kRows, TK);
             const uint64_t desc0 = sw128_matrix(sbase, kPlaneBytes / 2);
             int s = 0, buf = 0;
             uint32_t ph = 0, reuse = 1;
@@ -229,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int pl = 0; pl < P; ++pl)
 #pragma unroll
                             for (int k = 0; k < kStep / 16; ++k)   // 16 rows of 128 bytes
-                                mma_bf16<2>(tmem + (uint32_t)(buf * 256), d0 + (uint64_t)(pl * (kPlaneBytes >> 4)) + 128u * k,
+                                mma_bf16<2>(tmem + (uint32_t)(buf * TK), d0 + (uint64_t)(pl * (kPlaneBytes >> 4)) + 128u * k,
                                             dx + 128u * k, idesc, in > 0 || pl > 0 || k > 0);
                         mma_done<2>(done(s));
                         if (last) mma_done<2>(sums_full(buf));
@@ -260,13 +263,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp == 3) {
-            // each CTA's 128 columns of codes, and its rows' scales of their block
+            // each CTA's columns of codes (boxes of 128, of which the narrow tile uses 64),
+            // and the scales of the block that they lie in
             int a = 0;
             uint32_t ph = 1;
             for (int t = first; t < tiles; t += pairs) {
                 int nt, kt;
                 tile_of(t, p, nt, kt);
-                const int k0 = kt * kTile + rank * 128;
+                const int k0 = kt * TK + rank * (TK / 2);
                 const float* sc = p.scales + (min(k0, p.K - 1) >> 7) * p.s_col;
                 for (int i = 0; i < p.steps; ++i) {
                     wait(codes_read(a), ph);
@@ -324,7 +328,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int r = row_of(j);
                 const unsigned char* at = from + r * 128 + (chunk & 1) * 8;
                 code[j][0] = *reinterpret_cast<const uint2*>(at + (((chunk >> 1) ^ (r & 7)) << 4));
-                code[j][1] = *reinterpret_cast<const uint2*>(at + (((4 + (chunk >> 1)) ^ (r & 7)) << 4));
+                if constexpr (TK == 256)
+                    code[j][1] = *reinterpret_cast<const uint2*>(at + (((4 + (chunk >> 1)) ^ (r & 7)) << 4));
                 scale[j] = sc[r];
             }
 #pragma unroll
@@ -333,7 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const uint32_t at = x_at + (uint32_t)(s * L::STAGE + r * 128 + ((chunk ^ (r & 7)) << 4));
                 const uint64_t by = pack2(scale[j], scale[j]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < TK / 128; ++h) {
                     uint32_t o[4];
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
@@ -368,22 +373,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         const int q = warp & 3, half = (warp - 12) >> 2;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (TK / 2));
         const uint32_t free0 = in_cta(sums_empty(0), 0);
         int buf = 0;
         uint32_t ph = 0;
         for (int t = first; t < tiles; t += pairs) {
-            float acc[128];
+            float acc[TK / 2];
 #pragma unroll
-            for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
+            for (int c = 0; c < TK / 2; ++c) acc[c] = 0.0f;
             for (int i = 0; i < p.steps; i += L::SPAN) {
                 wait(sums_full(buf), ph);
                 __syncwarp();
                 tc_after();
 #pragma unroll
-                for (int c = 0; c < 128; c += 16) {
+                for (int c = 0; c < TK / 2; c += 16) {
                     uint64_t v[8];
-                    tmem_pairs(taddr + (uint32_t)(buf * 256 + c), v);
+                    tmem_pairs(taddr + (uint32_t)(buf * TK + c), v);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const float2 f = unpack2(v[k]);
@@ -399,11 +404,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             int nt, kt;
             tile_of(t, p, nt, kt);
-            const int64_t n = (int64_t)nt * kTile + rank * 128 + q * 32 + lane;
-            const int64_t k0 = (int64_t)kt * kTile + half * 128;
+            const int64_t n = (int64_t)nt * kRows + rank * 128 + q * 32 + lane;
+            const int64_t k0 = (int64_t)kt * TK + half * (TK / 2);
             if (n < p.N) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 16) {
+                for (int c = 0; c < TK / 2; c += 16) {
                     float v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
@@ -461,7 +466,7 @@ int terms_of(int type) { return type == kBf16 ? 1 : (type == kF16 ? 2 : 3); }
 int64_t term_ld(int64_t N) { return (N + 7) / 8 * 8; }
 int bytes_of(int type) { return type == kF32 ? 4 : 2; }
 
-template <int P, typename O>
+template <int P, int TK, typename O>
 cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
     Params p;
     p.scales = g.a.scales;
@@ -474,10 +479,10 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     p.N = (int)g.N;
     p.K = (int)g.K;
     p.steps = (int)((g.M + kStep - 1) / kStep);
-    p.tiles_n = (int)((g.N + kTile - 1) / kTile);
-    p.tiles_k = (int)((g.K + kTile - 1) / kTile);
+    p.tiles_n = (int)((g.N + kRows - 1) / kRows);
+    p.tiles_k = (int)((g.K + TK - 1) / TK);
     // a band's columns of x stay below 40 MB, well inside L2
-    int64_t band = ((int64_t)40 << 20) / (g.M * kTile);
+    int64_t band = ((int64_t)40 << 20) / (g.M * TK);
     band = band < 1 ? 1 : band;
     const int64_t bands = (p.tiles_k + band - 1) / band;
     p.band = (int)((p.tiles_k + bands - 1) / bands);
@@ -488,8 +493,8 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     if (!encode_rows(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, dy, g.N, P * g.M, ld * 2, kStep) ||
         !encode_codes(&mx, g.a.codes, g.a.cols, g.a.rows, g.a.ld, kStep))
         return cudaErrorInvalidValue;
-    const size_t smem = (size_t)Smem<P>::TOTAL + 1024;
-    auto kern = fp8_wgrad_kernel<P, O>;
+    const size_t smem = (size_t)Smem<P, TK>::TOTAL + 1024;
+    auto kern = fp8_wgrad_kernel<P, TK, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kLaunchRegs, ready);
     if (e != cudaSuccess) return e;
@@ -499,11 +504,21 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     return cudaLaunchKernelEx(&cfg.c, kern, p, map, mx);
 }
 
+template <int P, typename O>
+cudaError_t launch_tile(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
+    // rounds of tiles over the pairs of SMs, times a tile's time: 128 columns take
+    // 0.6 of what 256 do
+    const int64_t pairs = sm_count() / 2, rows = (g.N + kRows - 1) / kRows;
+    const int64_t wide = (rows * ((g.K + 255) / 256) + pairs - 1) / pairs;
+    const int64_t narrow = (rows * ((g.K + 127) / 128) + pairs - 1) / pairs;
+    return 10 * wide <= 6 * narrow ? launch_po<P, 256, O>(g, dy, ld, s) : launch_po<P, 128, O>(g, dy, ld, s);
+}
+
 template <int P>
 cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
-    if (g.out_type == kF16) return launch_po<P, __half>(g, dy, ld, s);
-    if (g.out_type == kBf16) return launch_po<P, __nv_bfloat16>(g, dy, ld, s);
-    return launch_po<P, float>(g, dy, ld, s);
+    if (g.out_type == kF16) return launch_tile<P, __half>(g, dy, ld, s);
+    if (g.out_type == kBf16) return launch_tile<P, __nv_bfloat16>(g, dy, ld, s);
+    return launch_tile<P, float>(g, dy, ld, s);
 }
 
 template <typename T, int P>
