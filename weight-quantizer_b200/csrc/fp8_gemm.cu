@@ -18,41 +18,60 @@ namespace {
 
 // ---- large products: pairs of CTAs ------------------------------------------------
 //
-// A pair of CTAs (two SMs) makes a 256 x 256 tile of y with tcgen05.mma of
-// cta_group::2: each CTA holds 128 rows of a and 128 of the tile's 256 columns of
-// w in shared memory, and 128 rows x 256 columns of the block's sums in tensor
-// memory, twice (512 columns), so that block b + 1 multiplies while block b is
-// read back. Bytes from L2 per block and CTA: 32 KB for 128 x 256 x 128 products,
-// half of what one CTA with a 128 x 128 tile would read.
+// A pair of CTAs (two SMs) makes a 256 x TN tile of y with tcgen05.mma of
+// cta_group::2: each CTA holds 128 rows of a and half of the tile's columns of w in
+// shared memory, and 128 rows x TN columns of a block's sums in tensor memory, as
+// often as fit (TN = 256 twice, TN = 128 four times), so that the next blocks
+// multiply while one is read back. Bytes from L2 per block and CTA at TN = 256: 32 KB
+// for 128 x 256 x 128 products.
 //
-// Warp 0 of each CTA loads (TMA, 128-byte swizzle: a block of 128 codes is one
-// swizzled row), warp 1 of the even CTA issues the MMAs of both, and eight
-// warps of each CTA hold the sums: warp e reads tensor-memory lanes 32 (e % 4)
-// .. + 31 (a lane is a row of y, so its scale is one register) and columns
-// 128 (e / 4) .. + 127 (one 128-column block, so sb is one value).
+// What bounds it: a block's hand-off. At TN = 256 a block takes 775 cycles, 512 of
+// them MMAs: a buffer is seen free by the issuer 230 cycles after its release, the
+// issue takes 100, the MMAs' latency is 300 beyond their time, and reading the sums
+// takes 320, with two buffers in flight. (Three buffers of 160 columns took the
+// summing warps 600 cycles for each 160 columns, more per column; four of 128
+// columns, which fill the SMs better when there are few tiles, take about 0.6 of the
+// wide tile's time.) Long products at full width also reach the board's power limit:
+// 4096 x 28672 x 8192 runs at 1.5 GHz and 990 W, 0.90 to 0.95 ms = 2.0 to 2.1 PFLOP/s.
 //
-// The transposed weight needs no copy: rows of 128 codes along y's columns are
-// the MMA's MN-major form of the same operand.
+// In each CTA warp 0 loads (TMA, 128-byte swizzle: a block of 128 codes is one
+// swizzled row) and warp 3 copies the scales. Warps 1 and 2 of the even CTA issue the
+// MMAs of both, alternate blocks: a wait on a barrier takes up to 200 cycles beside
+// the MMAs' own reads of shared memory, so one warp would spend a block's time on its
+// waits. Warps 4-11 of each CTA hold the sums: warp 4 + e reads tensor-memory lanes
+// 32 (e % 4) .. + 31 (a lane is a row of y, so its scale is one value) and half of the
+// columns (of one column block of w).
+//
+// The transposed weight needs no copy: rows of 128 codes along y's columns are the
+// MMA's MN-major form of the same operand.
 
-constexpr int kPairTile = 256;
-constexpr int kPairStages = 6;                      // even: each issuing warp has its own
+constexpr int kPairRows = 256;
 constexpr int kPairScaleSlots = 3;                  // blocks whose scales are on their way
 constexpr int kPairScaleBytes = (128 + 4) * 4;      // a's of the CTA's rows, w's of its two column blocks
 constexpr int kOutBytes = 4096;                     // a summing warp's part of y on its way out
 constexpr int kOperandBytes = 128 * 128;            // one operand of one CTA for one block
-constexpr int kPairStage = 2 * kOperandBytes;
 constexpr int kPairThreads = 384;
 constexpr int kPairLaunchRegs = 168, kPairCtlRegs = 56, kPairSumRegs = 224;
 static_assert(kPairCtlRegs + 2 * kPairSumRegs <= 3 * kPairLaunchRegs, "register split exceeds the launch's registers");
 
+// TN columns of y per tile: 256, or 128 where that fills the SMs better.
+template <bool WT, int TN>
 struct PairSmem {
-    static constexpr int OUT = kPairStages * kPairStage;
+    // a CTA's columns of w for one block: rows of 128 codes, or, of the transposed
+    // weight, 128 rows of the 128 codes that a box of the swizzle holds (64 of them
+    // used by the narrow tile)
+    static constexpr int W_ROWS = WT ? 128 : TN / 2;
+    static constexpr int STAGE = kOperandBytes + W_ROWS * 128;
+    static constexpr int STAGES = STAGE > 24576 ? 6 : 8;   // even: each issuing warp has its own
+    static constexpr int BUFS = 512 / TN;                  // even likewise
+    static_assert(BUFS <= STAGES, "a stage's barrier would lap the summing warps");
+    static constexpr int OUT = STAGES * STAGE;
     static constexpr int SCALES = OUT + 8 * kOutBytes;
     static constexpr int BAR = SCALES + kPairScaleSlots * kPairScaleBytes;
     // full and done per stage (done: the block's MMAs are over, so its operands
-    // may be replaced and its sums read); sums empty[2]
-    // per scale slot there, read
-    static constexpr int TMEM_SLOT = BAR + 8 * (2 * kPairStages + 2 + 2 * kPairScaleSlots);
+    // may be replaced and its sums read); sums empty per buffer; per scale slot
+    // there, read
+    static constexpr int TMEM_SLOT = BAR + 8 * (2 * STAGES + BUFS + 2 * kPairScaleSlots);
     static constexpr int FLAG = TMEM_SLOT + 8;
     static constexpr int TOTAL = TMEM_SLOT + 16;
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
@@ -71,7 +90,7 @@ struct PairParams {
     int tiles_m, tiles_n, band;
     bool tma_out;            // rows of out are 16-byte aligned
     int splits;              // parts of the inner blocks, each a tile's work for a pair of its own
-    float* part;             // [tile][split][rank] sums of 128 x 256
+    float* part;             // [tile][split][rank] sums of 128 x TN
     unsigned int* arrived;   // [tile][rank], zeroed before the launch
     unsigned int* fault;
 };
@@ -86,14 +105,14 @@ __device__ __forceinline__ void tile_of(int t, const PairParams& p, int& mt, int
     mt = b * p.band + (in - nt * bw);
 }
 
-// A warp's 32 rows (from m0) x 128 columns (from n0) of y out of its sums: a lane is
+// A warp's 32 rows (from m0) x C columns (from n0) of y out of its sums: a lane is
 // a row. By way of shared memory (128 bytes of 32 rows at a time, swizzled) and a TMA
 // store that ends at y's edges and drains while the next tile's blocks are summed:
 // stores from registers held the tile's hand-off for 4300 cycles, every CTA's 64 KB
 // at once.
-template <typename O>
+template <typename O, int C>
 __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap* map, uint32_t out, int lane,
-                                         int64_t m0, int64_t n0, const uint64_t (&acc)[64]) {
+                                         int64_t m0, int64_t n0, const uint64_t (&acc)[C / 2]) {
     constexpr int PER = 16 / (int)sizeof(O);      // values in 16 bytes
     constexpr int BOX = 8 * PER;                  // columns in 128 bytes
     const bool has_bias = p.bias != nullptr;
@@ -105,7 +124,7 @@ __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap*
     };
     if (p.tma_out) {
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += BOX) {
+        for (int c0 = 0; c0 < C; c0 += BOX) {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
 #pragma unroll
@@ -130,16 +149,17 @@ __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap*
     } else if (m0 + lane < p.M) {
         O* row = static_cast<O*>(p.out) + (m0 + lane) * p.ldo + n0;
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
+        for (int c = 0; c < C; ++c)
             if (n0 + c < p.N) row[c] = value(c);
     }
 }
 
-template <bool WT, bool SPLIT, typename O>
+template <bool WT, bool SPLIT, int TN, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     fp8_gemm_pair_kernel(const PairParams p, const __grid_constant__ CUtensorMap map_a,
                          const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y) {
-    using L = PairSmem;
+    using L = PairSmem<WT, TN>;
+    constexpr int NS = L::STAGES, NB = L::BUFS, C = TN / 2;   // C: columns of w of one CTA, and of a summing warp
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -148,17 +168,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int rank = (int)cluster_rank();
     auto bar = [&](int i) -> uint32_t { return sbase + L::BAR + 8u * (uint32_t)i; };
     auto full = [&](int s) { return bar(s); };
-    auto done = [&](int s) { return bar(kPairStages + s); };
-    auto sums_empty = [&](int b) { return bar(2 * kPairStages + b); };
-    auto scaled = [&](int c) { return bar(2 * kPairStages + 2 + c); };
-    auto scales_read = [&](int c) { return bar(2 * kPairStages + 2 + kPairScaleSlots + c); };
+    auto done = [&](int s) { return bar(NS + s); };
+    auto sums_empty = [&](int b) { return bar(2 * NS + b); };
+    auto scaled = [&](int c) { return bar(2 * NS + NB + c); };
+    auto scales_read = [&](int c) { return bar(2 * NS + NB + kPairScaleSlots + c); };
     launch_dependents();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPairStages; ++s) {
+        for (int s = 0; s < NS; ++s) {
             mbar_init(full(s), 1);     // the even CTA's: its own arrival plus both CTAs' bytes
             mbar_init(done(s), 1);
         }
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b)
             mbar_init(sums_empty(b), 16);   // the even CTA's: one arrival per summing warp of the pair
         for (int c = 0; c < kPairScaleSlots; ++c) {
             mbar_init(scaled(c), 32);
@@ -190,7 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairCtlRegs));
         if (warp == 0) {
-            // each CTA loads its 128 rows of a and its 128 columns of w; the
+            // each CTA loads its 128 rows of a and its columns of w; the
             // bytes count on the even CTA's barrier
             const uint32_t full0 = in_cta(full(0), 0);
             int s = 0;
@@ -198,21 +218,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int t = first; t < items; t += pairs) {
                 int mt, nt;
                 tile_of(t / splits, p, mt, nt);
-                const int m0 = mt * kPairTile + rank * 128, n0 = nt * kPairTile + rank * 128;
+                const int m0 = mt * kPairRows + rank * 128, n0 = nt * TN + rank * C;
                 const int b1 = to_block(t);
                 for (int b = from_block(t); b < b1; ++b) {
                     if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
                     __syncwarp();
                     if (elect_one()) {
                         const uint32_t f = full0 + 8u * (uint32_t)s;
-                        const uint32_t dst = sbase + (uint32_t)(s * kPairStage);
-                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
+                        const uint32_t dst = sbase + (uint32_t)(s * L::STAGE);
+                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * L::STAGE);
                         tma_box<2>(dst, &map_a, b * 128, m0, f);
                         if constexpr (WT) tma_box<2>(dst + kOperandBytes, &map_w, n0, b * 128, f);
                         else tma_box<2>(dst + kOperandBytes, &map_w, b * 128, n0, f);
                     }
                     __syncwarp();
-                    if (++s == kPairStages) {
+                    if (++s == NS) {
                         s = 0;
                         ph ^= 1u;
                     }
@@ -220,9 +240,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             // every copy this warp started has been read before the CTA goes
             // (a stage that was never filled passes at once)
-            for (int i = 0; i < kPairStages; ++i) {
+            for (int i = 0; i < NS; ++i) {
                 if (!mbar_wait_bounded(done(s), ph)) atomicOr(p.fault, 1u);
-                if (++s == kPairStages) {
+                if (++s == NS) {
                     s = 0;
                     ph ^= 1u;
                 }
@@ -231,31 +251,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             // even blocks by warp 1, odd ones by warp 2: a wait on a barrier takes
             // about 170 cycles beside the MMAs' own reads of shared memory, and one
             // warp's waits and its issue together take as long as a block's MMAs
-            constexpr uint32_t idesc = mma_idesc(0, false, WT, 256, 256);
+            constexpr uint32_t idesc = mma_idesc(0, false, WT, kPairRows, TN);
             const uint64_t desc0 = sw128_matrix(sbase);
-            const int buf = warp - 1;
-            const uint32_t d = tmem + (uint32_t)(buf * 256);
-            int s = buf;
-            uint32_t ph = 0;
-            for (int64_t i = buf; i < steps; i += 2) {
-                if (!faulted && !mbar_wait_bounded(full(s), ph)) give_up();
-                const uint64_t da = desc0 + (uint64_t)(s * (kPairStage >> 4));
+            int s = warp - 1, buf = warp - 1;
+            uint32_t ph = 0, free_ph = 1;   // (a fresh barrier's other phase counts as complete)
+            for (int64_t i = warp - 1; i < steps; i += 2) {
+                const uint64_t da = desc0 + (uint64_t)(s * (L::STAGE >> 4));
                 const uint64_t dw = da + (uint64_t)(kOperandBytes >> 4);
-                if (i >= 2 && !faulted && !mbar_wait_bounded(sums_empty(buf), (uint32_t)(((i >> 1) - 1) & 1)))
-                    give_up();
+                if (!try_wait_both(full(s), ph, sums_empty(buf), free_ph)) {
+                    if (!faulted && !mbar_wait_bounded(full(s), ph)) give_up();
+                    if (!faulted && !mbar_wait_bounded(sums_empty(buf), free_ph)) give_up();
+                }
                 __syncwarp();
                 tc_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)   // 32 codes: 32 bytes of a row, or 32 rows of 128 bytes
-                        mma_f8<2>(d, da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
+                        mma_f8<2>(tmem + (uint32_t)(buf * TN), da + 2u * k, dw + (WT ? 256u : 2u) * k, idesc, k > 0);
                     mma_done<2>(done(s));
                 }
                 __syncwarp();
                 s += 2;
-                if (s >= kPairStages) {
-                    s = buf;
+                if (s >= NS) {
+                    s -= NS;
                     ph ^= 1u;
+                }
+                buf += 2;
+                if (buf >= NB) {
+                    buf -= NB;
+                    free_ph ^= 1u;
                 }
             }
         } else if (warp == 3) {
@@ -267,10 +291,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int t = first; t < items; t += pairs) {
                 int mt, nt;
                 tile_of(t / splits, p, mt, nt);
-                const int64_t m0 = (int64_t)mt * kPairTile + rank * 128 + lane;
+                const int64_t m0 = (int64_t)mt * kPairRows + rank * 128 + lane;
                 const int b0 = from_block(t), b1 = to_block(t);
                 const float* sa = p.sa + m0 * p.sa_row + b0 * p.sa_col;
-                const float* sw = p.sw + min(2 * nt + (lane & 1), (p.N - 1) >> 7) * p.sw_n + b0 * p.sw_k;
+                const float* sw = p.sw + min((nt * TN + (lane & 1) * C) >> 7, (p.N - 1) >> 7) * p.sw_n + b0 * p.sw_k;
                 for (int b = b0; b < b1; ++b) {
                     if (!faulted && !mbar_wait_bounded(scales_read(c), ph)) give_up();
                     __syncwarp();
@@ -295,37 +319,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairSumRegs));
         const int q = warp & 3, half = (warp - 4) >> 2;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * C);
         const uint32_t free0 = in_cta(sums_empty(0), 0);
+        int s = 0, c = 0;
         int64_t i = 0;
-        int s = 0;
-        uint32_t ph = 0;
-        int c = 0;
-        uint32_t cph = 0;
+        uint32_t ph = 0, cph = 0;
         for (int t = first; t < items; t += pairs) {
-            int mt, nt;
-            tile_of(t / splits, p, mt, nt);
             const int b0 = from_block(t), b1 = to_block(t);
-            uint64_t acc[64];
+            uint64_t acc[C / 2];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = 0;
-            for (int b = b0; b < b1; ++b, ++i) {
-                const int buf = (int)(i & 1);
-                const uint32_t from = taddr + (uint32_t)(buf * 256);
-                uint64_t v[32];
+            for (int k = 0; k < C / 2; ++k) acc[k] = 0;
+            for (int b = b0; b < b1; ++b) {
                 if (!try_wait_both(done(s), ph, scaled(c), cph)) {
                     if (!faulted && !mbar_wait_bounded(scaled(c), cph)) give_up();
                     if (!faulted && !mbar_wait_bounded(done(s), ph)) give_up();
                 }
+                const int buf = (int)(i & (NB - 1));
                 __syncwarp();
                 tc_after();
                 const float* scales = reinterpret_cast<const float*>(smem + L::SCALES + c * kPairScaleBytes);
                 const float sc = scales[q * 32 + lane] * scales[128 + half];
                 const uint64_t sc2 = pack2(sc, sc);
+                const uint32_t from = taddr + (uint32_t)(buf * TN);
+                uint64_t v[32];
                 tmem_pairs(from, v);
+                if constexpr (C == 128) {   // 64 columns at a time, for the registers
 #pragma unroll
-                for (int c = 0; c < 32; ++c) fma2(acc[c], v[c], sc2);
-                tmem_pairs(from + 64u, v);
+                    for (int k = 0; k < 32; ++k) fma2(acc[k], v[k], sc2);
+                    tmem_pairs(from + 64u, v);
+                }
                 tc_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -333,8 +355,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     mbar_arrive(scales_read(c));
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) fma2(acc[32 + k], v[k], sc2);
-                if (++s == kPairStages) {
+                for (int k = 0; k < 32; ++k) fma2(acc[C / 2 - 32 + k], v[k], sc2);
+                ++i;
+                if (++s == NS) {
                     s = 0;
                     ph ^= 1u;
                 }
@@ -347,13 +370,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if constexpr (SPLIT) {
                 // the item's sums go to its slot, [column / 4][row][4]; the last of the
                 // tile's items adds them in order
-                const int64_t lane_at = ((int64_t)half * 32 * 128 + q * 32 + lane) * 4;
-                constexpr int64_t SLOT = 128 * 256;
+                const int64_t lane_at = ((int64_t)half * (C / 4) * 128 + q * 32 + lane) * 4;
+                constexpr int64_t SLOT = 128 * TN;
                 float4* mine = reinterpret_cast<float4*>(p.part + ((int64_t)t * 2 + rank) * SLOT + lane_at);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const float2 f = unpack2(acc[2 * c]), g = unpack2(acc[2 * c + 1]);
-                    mine[c * 128] = make_float4(f.x, f.y, g.x, g.y);
+                for (int k = 0; k < C / 4; ++k) {
+                    const float2 f = unpack2(acc[2 * k]), g = unpack2(acc[2 * k + 1]);
+                    mine[k * 128] = make_float4(f.x, f.y, g.x, g.y);
                 }
                 __threadfence();
                 named_barrier(1, 256);
@@ -367,24 +390,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (write) {
                     __threadfence();
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) acc[c] = 0;
+                    for (int k = 0; k < C / 2; ++k) acc[k] = 0;
                     const uint64_t one = pack2(1.0f, 1.0f);
 #pragma unroll 1
                     for (int sp = 0; sp < splits; ++sp) {
                         const float4* src = reinterpret_cast<const float4*>(
                             p.part + (((int64_t)tile * splits + sp) * 2 + rank) * SLOT + lane_at);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const float4 f = __ldcg(src + c * 128);
-                            fma2(acc[2 * c], pack2(f.x, f.y), one);
-                            fma2(acc[2 * c + 1], pack2(f.z, f.w), one);
+                        for (int k = 0; k < C / 4; ++k) {
+                            const float4 f = __ldcg(src + k * 128);
+                            fma2(acc[2 * k], pack2(f.x, f.y), one);
+                            fma2(acc[2 * k + 1], pack2(f.z, f.w), one);
                         }
                     }
                 }
             }
+            int mt, nt;
+            tile_of(t / splits, p, mt, nt);
             if (write)
-                put_tile<O>(p, &map_y, sbase + (uint32_t)(L::OUT + (warp - 4) * kOutBytes), lane,
-                            (int64_t)mt * kPairTile + rank * 128 + q * 32, (int64_t)nt * kPairTile + half * 128, acc);
+                put_tile<O, C>(p, &map_y, sbase + (uint32_t)(L::OUT + (warp - 4) * kOutBytes), lane,
+                            (int64_t)mt * kPairRows + rank * 128 + q * 32, (int64_t)nt * TN + half * C, acc);
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -749,28 +774,45 @@ __global__ void fill_rows_kernel(O* out, int64_t M, int64_t N, int64_t ldo, cons
 // ---- plan ----
 
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
-int64_t pair_tiles(int64_t M, int64_t N) {
-    return ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile);
+int64_t pair_tiles(int64_t M, int64_t N, int tn) { return ((M + kPairRows - 1) / kPairRows) * ((N + tn - 1) / tn); }
+// The tile's columns, the parts that its inner blocks are cut into, and the time, in
+// microseconds, by a model fitted to both on weights of 2304 x 768 to 28672 x 8192 at
+// 65 to 4096 rows: 5, kWideUs or kNarrowUs for each round of blocks over the pairs of
+// SMs (or the weights at 5.5 TB/s, if that is longer), and 16 + 2 for each part that
+// a tile's blocks are cut into (at least four blocks, one pair each) where there are
+// at most half as many tiles as pairs.
+constexpr double kWideUs = 0.43, kNarrowUs = 0.26;
+struct PairPlan {
+    int tn, splits;
+    double us;
+};
+PairPlan pair_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t pairs = sm_count() / 2, blocks = (K + 127) / 128;
+    const double stream = (double)N * (double)K / 5.5e6;
+    PairPlan best{256, 1, 1e30};
+    for (int tn = 256; tn >= 128; tn -= 128) {
+        const int64_t tiles = pair_tiles(M, N, tn);
+        int64_t most = pairs / tiles;
+        if (most > blocks / 4) most = blocks / 4;
+        if (most > 8) most = 8;
+        for (const int64_t n : {(int64_t)1, most < 1 ? (int64_t)1 : most}) {
+            const int64_t rounds = (tiles * n + pairs - 1) / pairs;
+            const double run = (double)(rounds * ((blocks + n - 1) / n)) * (tn == 256 ? kWideUs : kNarrowUs);
+            const double us = 5.0 + (run > stream ? run : stream) + (n > 1 ? 16.0 + 2.0 * (double)n : 0.0);
+            if (us < best.us) best = PairPlan{tn, (int)n, us};
+        }
+    }
+    return best;
 }
-// Few tiles (at most half as many as pairs of SMs): their inner blocks are cut into
-// parts of at least four, one pair each, where that saves more than the parts' sums
-// cost (16 + 2 each, in microseconds, at 0.43 per block: 129 x 4096 x 11008 in four
-// parts 31, whole 37; 129 x 4096 x 4096 in four parts 24, whole 18).
-constexpr int64_t kPairMaxSplits = 8;
-int pair_splits(int64_t M, int64_t N, int64_t K) {
-    const int64_t tiles = pair_tiles(M, N), blocks = (K + 127) / 128;
-    int64_t n = sm_count() / 2 / tiles;
-    if (n > blocks / 4) n = blocks / 4;
-    if (n > kPairMaxSplits) n = kPairMaxSplits;
-    if (n < 2 || 0.43 * (double)(blocks - (blocks + n - 1) / n) < 16.0 + 2.0 * (double)n) return 1;
-    return (int)n;
+size_t pair_arrived_bytes(int64_t M, int64_t N, int64_t K) {
+    return round_up((size_t)pair_tiles(M, N, pair_plan(M, N, K).tn) * 2 * 4);
 }
-size_t pair_arrived_bytes(int64_t M, int64_t N) { return round_up((size_t)pair_tiles(M, N) * 2 * 4); }
 size_t pair_part_bytes(int64_t M, int64_t N, int64_t K) {
-    return (size_t)pair_tiles(M, N) * pair_splits(M, N, K) * 2 * 128 * 256 * 4;
+    const PairPlan plan = pair_plan(M, N, K);
+    return (size_t)pair_tiles(M, N, plan.tn) * plan.splits * 2 * 128 * plan.tn * 4;
 }
 
-template <bool WT, bool SPLIT, typename O>
+template <bool WT, bool SPLIT, int TN, typename O>
 cudaError_t launch_pair_o(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
     PairParams p;
     p.sa = g.a.scales;
@@ -786,23 +828,23 @@ cudaError_t launch_pair_o(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     p.M = (int)g.M;
     p.N = (int)g.N;
     p.blocks = (int)((g.K + 127) / 128);
-    p.tiles_m = (int)((g.M + kPairTile - 1) / kPairTile);
-    p.tiles_n = (int)((g.N + kPairTile - 1) / kPairTile);
+    p.tiles_m = (int)((g.M + kPairRows - 1) / kPairRows);
+    p.tiles_n = (int)((g.N + TN - 1) / TN);
     // the rows of a band stay below 40 MB, well inside L2
-    const int64_t per_tile = (int64_t)kPairTile * p.blocks * 128;
+    const int64_t per_tile = (int64_t)kPairRows * p.blocks * 128;
     int64_t band = ((int64_t)40 << 20) / per_tile;
     band = band < 1 ? 1 : band;
     const int64_t bands = (p.tiles_m + band - 1) / band;
     p.band = (int)((p.tiles_m + bands - 1) / bands);
     p.splits = splits;
     p.arrived = static_cast<unsigned int*>(workspace);
-    p.part = SPLIT ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pair_arrived_bytes(g.M, g.N))
+    p.part = SPLIT ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pair_arrived_bytes(g.M, g.N, g.K))
                    : nullptr;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
     CUtensorMap ma, mw, my = {};
     if (!encode_codes(&ma, g.a.codes, g.a.cols, g.a.rows, g.a.ld, 128) ||
-        !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, 128))
+        !encode_codes(&mw, g.w.codes, g.w.cols, g.w.rows, g.w.ld, PairSmem<WT, TN>::W_ROWS))
         return cudaErrorInvalidValue;
     constexpr CUtensorMapDataType DT = sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : std::is_same<O, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
@@ -810,8 +852,8 @@ cudaError_t launch_pair_o(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     const int64_t out_pitch = g.M > 1 ? g.ldo * (int64_t)sizeof(O) : (g.N * (int64_t)sizeof(O) + 15) / 16 * 16;
     p.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && out_pitch % 16 == 0 &&
                 encode_rows(&my, DT, (int)sizeof(O), g.out, g.N, g.M, out_pitch, 32);
-    const size_t smem = (size_t)PairSmem::TOTAL + 1024;
-    auto kern = fp8_gemm_pair_kernel<WT, SPLIT, O>;
+    const size_t smem = (size_t)PairSmem<WT, TN>::TOTAL + 1024;
+    auto kern = fp8_gemm_pair_kernel<WT, SPLIT, TN, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kPairLaunchRegs, ready);
     if (e != cudaSuccess) return e;
@@ -822,22 +864,25 @@ cudaError_t launch_pair_o(const Fp8Gemm& g, int splits, void* workspace, cudaStr
     return cudaLaunchKernelEx(&cfg.c, kern, p, ma, mw, my);
 }
 
-template <bool WT, bool SPLIT>
+template <bool WT, bool SPLIT, int TN>
 cudaError_t launch_pair_s(const Fp8Gemm& g, int splits, void* workspace, cudaStream_t s) {
-    if (g.out_type == kF16) return launch_pair_o<WT, SPLIT, __half>(g, splits, workspace, s);
-    if (g.out_type == kBf16) return launch_pair_o<WT, SPLIT, __nv_bfloat16>(g, splits, workspace, s);
-    return launch_pair_o<WT, SPLIT, float>(g, splits, workspace, s);
+    if (g.out_type == kF16) return launch_pair_o<WT, SPLIT, TN, __half>(g, splits, workspace, s);
+    if (g.out_type == kBf16) return launch_pair_o<WT, SPLIT, TN, __nv_bfloat16>(g, splits, workspace, s);
+    return launch_pair_o<WT, SPLIT, TN, float>(g, splits, workspace, s);
 }
 
 template <bool WT>
 cudaError_t launch_pair(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
-    const int splits = pair_splits(g.M, g.N, g.K);
-    if (splits == 1) return launch_pair_s<WT, false>(g, 1, nullptr, s);
+    const PairPlan plan = pair_plan(g.M, g.N, g.K);
+    if (plan.splits == 1)
+        return plan.tn == 256 ? launch_pair_s<WT, false, 256>(g, 1, nullptr, s)
+                              : launch_pair_s<WT, false, 128>(g, 1, nullptr, s);
     if (!prepared) {
-        cudaError_t e = cudaMemsetAsync(workspace, 0, pair_arrived_bytes(g.M, g.N), s);
+        cudaError_t e = cudaMemsetAsync(workspace, 0, pair_arrived_bytes(g.M, g.N, g.K), s);
         if (e != cudaSuccess) return e;
     }
-    return launch_pair_s<WT, true>(g, splits, workspace, s);
+    return plan.tn == 256 ? launch_pair_s<WT, true, 256>(g, plan.splits, workspace, s)
+                          : launch_pair_s<WT, true, 128>(g, plan.splits, workspace, s);
 }
 
 // ---- few rows: plan ----
@@ -865,26 +910,17 @@ size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
 }
 size_t few_arrived_bytes(int64_t N) { return round_up((size_t)few_tiles(N) * 4); }
 
-// Which of the two kernels: the shorter by this model, in microseconds, fitted to
-// both on weights of 2304 x 768 to 28672 x 8192 at 1 to 128 rows (from memory, not
-// L2). Pairs: 5, and 0.43 for each round of blocks, or the weights at 5.5 TB/s if
-// that is longer; parts of tiles cost 12 + 2 each. Few rows: 8, a unit's time for
-// each unit of a CTA's run, and the CTAs that share a tile. Measured, pairs / few:
-// 28672 x 8192 at 16 rows 60 / 48, at 64 rows 66 / 58, at 128 rows 69 / 78;
-// 11008 x 4096 at 64 rows 19 / 25; 4096 x 11008 at 64 rows 31 / 24; 2304 x 768 6 / 8.
-double pair_us(int64_t M, int64_t N, int64_t K) {
-    const int64_t s = pair_splits(M, N, K), pairs = sm_count() / 2, blocks = (K + 127) / 128;
-    const double rounds = (double)((pair_tiles(M, N) * s + pairs - 1) / pairs);
-    const double run = rounds * (double)((blocks + s - 1) / s) * 0.43, stream = (double)N * (double)K / 5.5e6;
-    return 5.0 + (run > stream ? run : stream) + (s > 1 ? 12.0 + 2.0 * (double)s : 0.0);
-}
+// Which of the two kernels: the shorter by the pairs' model above and this one, from
+// memory, not L2: 8, a unit's time for each unit of a CTA's run, and the CTAs that
+// share a tile. Measured, wide pairs / few rows: 28672 x 8192 at 16 rows 60 / 48, at 64
+// rows 66 / 58; 11008 x 4096 at 64 rows 19 / 25; 2304 x 768 6 / 8.
 double few_us(int64_t M, int64_t N, int64_t K) {
     const int64_t blocks = (K + 127) / 128, units = few_tiles(N) * blocks;
     const double run = (double)units / (double)few_ctas(N, K, few_resident(M));
     const double shared = (double)blocks / run;   // CTAs on a tile
     return 8.0 + run * (M <= 32 ? 0.86 : 0.54) + (shared > 1.0 ? shared * (M <= 16 ? 0.5 : (M <= 32 ? 0.7 : 1.2)) : 0.0);
 }
-bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kFewMaxRows && few_us(M, N, K) <= pair_us(M, N, K); }
+bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kFewMaxRows && few_us(M, N, K) <= pair_plan(M, N, K).us; }
 
 template <int BN, bool WT, typename O>
 cudaError_t launch_few_o(const Fp8Gemm& g, const FewParams& p, cudaStream_t s) {
@@ -947,12 +983,12 @@ cudaError_t launch_few(const Fp8Gemm& g, void* workspace, bool prepared, cudaStr
 
 size_t fp8_gemm_zeroed_bytes(int64_t M, int64_t N, int64_t K) {
     if (few_rows(M, N, K)) return few_arrived_bytes(N);
-    return pair_splits(M, N, K) > 1 ? pair_arrived_bytes(M, N) : 0;
+    return pair_plan(M, N, K).splits > 1 ? pair_arrived_bytes(M, N, K) : 0;
 }
 
 size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (few_rows(M, N, K)) return few_arrived_bytes(N) + few_part_bytes(M, N, K);
-    return pair_splits(M, N, K) > 1 ? pair_arrived_bytes(M, N) + pair_part_bytes(M, N, K) : 0;
+    return pair_plan(M, N, K).splits > 1 ? pair_arrived_bytes(M, N, K) + pair_part_bytes(M, N, K) : 0;
 }
 
 cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
