@@ -357,6 +357,8 @@ WQ_API int wq_dequant_gemm_f32_multi(const float* x, int64_t B, int64_t K,
 /* 16-byte boundary and ld is a multiple of 16 (pad the rows; what the       */
 /* padding holds is not read as a value). Sums are held in fp32; every       */
 /* result is rounded once to its type and the same on every call.            */
+/* Workspaces are 256-byte aligned device memory of the queried size (none   */
+/* where that is 0), WQ_E_WORKSPACE otherwise, and serve one call at a time. */
 /* ------------------------------------------------------------------------ */
 enum wq_dtype { WQ_F32 = 0, WQ_F16 = 1, WQ_BF16 = 2 };
 

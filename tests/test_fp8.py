@@ -150,6 +150,26 @@ def test_product_c_refusals(wq) -> None:
     assert wg(N=0, dw=None) == 0 and wg(K=0, dw=None) == 0
 
 
+def test_workspace_alignment_c_refusals(wq) -> None:
+    """Workspaces that are needed and not 256-byte aligned, or too small, are refused by each entry point."""
+    lib = wq._kernels.library()
+    need = lib.wq_fp8_gemm_workspace_bytes(1, 4096, 8192)
+    assert need > 0
+
+    def g(ws, nws=need):  # type: ignore[no-untyped-def]
+        return lib.wq_fp8_gemm(P, 1, 8192, 8192, P, 64, 1, P, 4096, 8192, 8192, P, 64, 1, 0, None, 0, P, 2, 4096, ws,
+                               nws, None)
+
+    assert g(ctypes.c_void_p(256 + 16)) == 12 and g(None) == 12 and g(P, need - 1) == 12
+    need_w = lib.wq_fp8_weight_grad_workspace_bytes(4, 8, 256, 0)
+    assert need_w > 0
+
+    def wg(ws, nws=need_w):  # type: ignore[no-untyped-def]
+        return lib.wq_fp8_weight_grad(P, 0, 4, 8, 8, P, 256, 256, P, 2, 1, P, 0, 256, 0, ws, nws, None)
+
+    assert wg(ctypes.c_void_p(256 + 128)) == 12 and wg(None) == 12 and wg(P, need_w - 1) == 12
+
+
 def test_status_messages(wq) -> None:
     msg = wq._kernels.status_message
     assert msg(23) == "element type must be fp32, fp16 or bf16"

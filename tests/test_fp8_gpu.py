@@ -286,6 +286,26 @@ def test_product_scale_range(wq, cuda) -> None:
             assert bool(((y.double() - ref).abs() <= bound).all()), (rows, sa, sw)
 
 
+def test_offsets_past_32_bits(wq, cuda) -> None:
+    """An operand of more than 2^31 codes: its last rows as by themselves, in the quantizer, the product and the
+    weight gradient."""
+    rows, cols = 263_000, 8200
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=cuda)
+    x[-300:] = rand((300, cols), 1, torch.bfloat16)
+    q, last = wq.quantize_fp8(x), wq.quantize_fp8(x[-300:])
+    assert rows * cols > 2 ** 31
+    assert torch.equal(q.codes[-300:].view(torch.uint8), last.codes.view(torch.uint8))
+    assert torch.equal(q.scales[-300:], last.scales) and bool((q.scales[:-300] == 1).all())
+    del x
+    w = wq.quantize_fp8(rand((100, cols), 2, torch.bfloat16, 0.02), block_rows=128)
+    y = wq.fp8_gemm(q, w, out_dtype=torch.float32)
+    check_product(y[-300:], values64(last), values64(w).t())
+    assert bool((y[:-300] == 0).all())
+    dy = torch.ones(rows, 9, dtype=torch.bfloat16, device=cuda)
+    dw = wq.fp8_weight_grad(dy, q)
+    check_product(dw, dy[-300:].double().t(), values64(last))
+
+
 # ---- the weight gradient ---------------------------------------------------------------
 
 

@@ -573,6 +573,12 @@ int wq_chol_inverse_upper_f64(const double* a, int64_t n, int64_t lda, double* u
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
 
+// The workspaces hold 16-byte partial sums and the targets of asynchronous
+// copies: 256-byte alignment, what an allocator gives.
+static bool fp8_workspace_ok(const void* workspace, size_t bytes, size_t need) {
+    return need == 0 || (workspace != nullptr && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0);
+}
+
 static bool fp8_type_ok(int t) { return t == WQ_F32 || t == WQ_F16 || t == WQ_BF16; }
 
 int wq_fp8_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int block_rows,
@@ -640,7 +646,7 @@ int wq_fp8_gemm(const uint8_t* a, int64_t M, int64_t K, int64_t lda, const float
     if (out == nullptr) return WQ_E_NULL;
     if (K > 0 && (a == nullptr || a_scales == nullptr || w == nullptr || w_scales == nullptr)) return WQ_E_NULL;
     const size_t need = wq_fp8_gemm_workspace_bytes(M, N, K);
-    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
+    if (!fp8_workspace_ok(workspace, workspace_bytes, need)) return WQ_E_WORKSPACE;
     const wq::Fp8Operand ao{a, M, K, lda, a_scales, as_row, as_col, 1};
     const wq::Fp8Operand wo{w, w_rows, w_cols, ldw, w_scales, ws_row, ws_col, wq::kFp8Block};
     const wq::Fp8Gemm g{ao, wo, transpose ? 1 : 0, M, N, K, bias, bias_type, out, out_type, ldo};
@@ -674,8 +680,7 @@ int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_t ldx, 
     if (out == nullptr) return WQ_E_NULL;
     if (K > 0 && (x == nullptr || w == nullptr || w_scales == nullptr)) return WQ_E_NULL;
     const size_t need = wq_fp8_linear_workspace_bytes(M, N, K);
-    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
-    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return WQ_E_WORKSPACE;
+    if (!fp8_workspace_ok(workspace, workspace_bytes, need)) return WQ_E_WORKSPACE;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     float* scales = reinterpret_cast<float*>(codes + fp8_codes_bytes(M, K));
@@ -711,7 +716,7 @@ int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_
     if (dw == nullptr) return WQ_E_NULL;
     if (M > 0 && (dy == nullptr || codes == nullptr || scales == nullptr)) return WQ_E_NULL;
     const size_t need = wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type);
-    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return WQ_E_WORKSPACE;
+    if (!fp8_workspace_ok(workspace, workspace_bytes, need)) return WQ_E_WORKSPACE;
     const wq::Fp8Operand ao{codes, M, K, ld, scales, s_row, s_col, 1};
     const wq::Fp8WeightGrad g{dy, dy_type, ldy, ao, M, N, K, dw, dw_type, ldw, accumulate ? 1 : 0};
     cudaError_t e = wq::launch_fp8_weight_grad(g, workspace, static_cast<cudaStream_t>(stream));

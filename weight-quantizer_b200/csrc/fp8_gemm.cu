@@ -423,19 +423,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // ---- few rows: weights stream by, the work split evenly ------------------------------
 //
 // With few rows of a the bound is the weights' bytes (and, once they are in L2, the
-// latency of each block). One CTA per SM; the MMA's rows (tensor-memory lanes) are
-// 128 rows of w, its columns `bn` <= BN rows of a. The work is cut into units of 128
-// rows of w x one block, and every CTA takes an equal run of them, wherever tiles
-// begin or end (224 row tiles on 148 SMs would leave a quarter of them idle in the
-// second round). A CTA that holds a whole tile writes y; the others put their sums
-// into the workspace, and the last to arrive at a tile adds them in CTA order (a
-// fixed order, whoever is last) and writes y.
+// latency of each block). The MMA's rows (tensor-memory lanes) are 128 rows of w, its
+// columns `bn` <= BN rows of a. The work is cut into units of 128 rows of w x one
+// block, and every CTA takes an equal run of them, wherever tiles begin or end (224
+// row tiles on 148 SMs would leave a quarter of them idle in the second round). A CTA
+// that holds a whole tile writes y; the others put their sums into the workspace, and
+// the last to arrive at a tile adds them in CTA order (a fixed order, whoever is last)
+// and writes y.
 //
-// Warp 0 loads units (TMA) into a ring that spans ten of them (180 KB in flight per
-// SM); warps 1 and 2 issue the MMAs of even and odd units; warp 3 copies the unit's
+// Two CTAs per SM for up to 32 rows, each with a ring of four units, one with eight
+// for more: 148-192 KB in flight per SM either way. Warp 0 loads units (TMA) into the
+// ring; warps 1 and 2 issue the MMAs of even and odd units; warp 3 copies the unit's
 // scales (asynchronous 4-byte copies); the other warps add each unit's sums, times
-// the scales, to registers. Up to eight units' sums are in tensor memory, so no
-// hand-off waits for another.
+// the scales, to registers. As many units' sums as the ring has stages fit in tensor
+// memory, so no hand-off waits for another.
+//
+// One row through 28672 x 8192: 46.4 us; reading its 235 MB takes 35.9 us at the
+// measured copy rate, and this ring of TMA loads without the products 37-41 us.
 
 template <int BN>
 struct Few {

@@ -6,7 +6,8 @@
 // an operand. With power-of-two scales (quantize_fp8's) code * scale is exact in
 // bf16, and dy is bf16 already, or is split into bf16 terms that add up to it (two
 // for fp16, three for fp32): every product is exact. Other scales' code * scale is
-// rounded to bf16 (half a step 2^-9 of each value), the operand type's only choice.
+// rounded to bf16 (by at most 2^-8 of each value), the only 16-bit operand type with
+// the scales' range.
 //
 // Sums over 512 rows (256 and 128 with two and three terms) stay in tensor memory,
 // then they are added to fp32 registers: the tensor core's own additions cut off what
@@ -30,7 +31,7 @@ namespace {
 // e4m3 -> fp16 -> fp32, times the row's scale, to bf16 in the swizzled tile; a lane
 // takes eight codes of each 64 columns, which are one 16-byte chunk of that tile, so
 // that eight lanes fill a row without bank conflicts. Eight more warps
-// (12-19) add the finished sums of 512 rows to their registers: a lane is a row of
+// (12-19) add the finished sums of a span to their registers: a lane is a row of
 // dw, a warp has TK / 2 columns. TK is 256, or 128 where that fills the SMs better
 // (a step of the narrow tile takes a little over half as long; 2304 x 768 is 27 wide
 // tiles for 74 pairs, or 54 narrow ones).
