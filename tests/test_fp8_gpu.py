@@ -331,6 +331,34 @@ def test_weight_grad_long(wq, cuda) -> None:
         assert float((dw.double() - ref).norm() / ref.norm()) <= 100 * 2.0 ** -24
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(8192, 128, 128), (4100, 300, 520), (8192, 1, 1), (3001, 777, 130)])
+def test_weight_grad_rows_in_parts(wq, cuda, M: int, N: int, K: int, dtype) -> None:
+    """Many rows and few tiles: the rows are summed in parts by several pairs of SMs. Run twice, the same bits; a
+    strided output that is added to; a replayed graph on new values."""
+    dy = rand((M, N), 1, dtype, 1e-2)
+    x = wq.quantize_fp8(rand((M, K), 2, torch.bfloat16))
+    dw = wq.fp8_weight_grad(dy, x)
+    check_product(dw, dy.double().t(), values64(x))
+    for _ in range(20):
+        assert torch.equal(wq.fp8_weight_grad(dy, x), dw)
+    big = torch.full((N + 2, K + 9), 0.25, device=cuda)
+    got = wq.fp8_weight_grad(dy, x, out=big[1:-1, 4:4 + K], accumulate=True)
+    ref = dw.double() + 0.25
+    assert bool(((got.double() - ref).abs() <= 2.0 ** -24 * ref.abs()).all())
+    big[1:-1, 4:4 + K] = 0.25
+    assert bool((big == 0.25).all())
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        again = wq.fp8_weight_grad(dy, x)
+    for seed in (3, 4, 5):
+        dy.copy_(rand((M, N), seed, dtype, 1e-2))
+        graph.replay()
+        assert torch.equal(again, wq.fp8_weight_grad(dy, x))
+
+
 def test_weight_grad_layouts_and_accumulate(wq, cuda) -> None:
     base = rand((90, 400), 1, torch.bfloat16)
     x = wq.quantize_fp8(rand((90, 515), 2))

@@ -34,7 +34,9 @@ namespace {
 // (12-19) add the finished sums of a span to their registers: a lane is a row of
 // dw, a warp has TK / 2 columns. TK is 256, or 128 where that fills the SMs better
 // (a step of the narrow tile takes a little over half as long; 2304 x 768 is 27 wide
-// tiles for 74 pairs, or 54 narrow ones).
+// tiles for 74 pairs, or 54 narrow ones). Where even the narrow tiles are fewer than
+// half of the pairs, the rows are cut into parts (SPLIT): each pair writes its part's
+// sums to the workspace, and the last to arrive at a tile adds them in order.
 
 constexpr int kRows = 256;                     // rows of dw in a tile
 constexpr int kStep = 64;                      // rows of dy and x per step
@@ -61,6 +63,7 @@ struct Smem {
     // full and done per stage; the odd CTA's x^ ready per stage; codes there and read;
     // sums full[2], empty[2]
     static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 2 * kAhead + 4);
+    static constexpr int FLAG = TMEM_SLOT + 8;
     static constexpr int TOTAL = TMEM_SLOT + 16;
     static_assert(STAGES >= 2, "the MMAs of one step run while the next is made");
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
@@ -75,6 +78,9 @@ struct Params {
     int M, N, K, steps;
     int tiles_n, tiles_k, band;
     bool wide_out;
+    int splits;              // parts of the rows
+    float* part;             // [tile][part][rank] sums of 128 x TK
+    unsigned int* arrived;   // per tile and rank, zeroed before the launch
     unsigned int* fault;
 };
 
@@ -114,7 +120,7 @@ __device__ __forceinline__ void put16(O* row, int64_t c, int64_t k, bool wide, c
     }
 }
 
-template <int P, int TK, typename O>
+template <int P, int TK, bool SPLIT, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy,
                      const __grid_constant__ CUtensorMap map_x) {
@@ -161,8 +167,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grid_wait();   // nothing above reads global memory
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::TMEM_SLOT);
     const int pairs = (int)gridDim.x >> 1, first = (int)blockIdx.x >> 1;
-    const int tiles = p.tiles_n * p.tiles_k;
-    const int mine = first < tiles ? (tiles - 1 - first) / pairs + 1 : 0;
+    // an item is a part of a tile's steps
+    const int splits = SPLIT ? p.splits : 1;
+    const int items = p.tiles_n * p.tiles_k * splits;
+    auto from_step = [&](int item) -> int {
+        return SPLIT ? (int)((int64_t)(item % splits) * p.steps / splits) : 0;
+    };
+    auto to_step = [&](int item) -> int {
+        return SPLIT ? (int)((int64_t)(item % splits + 1) * p.steps / splits) : p.steps;
+    };
+    int64_t total = 0;   // this pair's steps
+    if constexpr (SPLIT)
+        for (int t = first; t < items; t += pairs) total += to_step(t) - from_step(t);
+    else
+        total = first < items ? (int64_t)((items - 1 - first) / pairs + 1) * p.steps : 0;
     bool faulted = false;
     auto wait = [&](uint32_t b, uint32_t parity) {
         if (!faulted && !mbar_wait_bounded(b, parity)) {
@@ -177,11 +195,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t full0 = in_cta(full(0), 0);
             int s = 0;
             uint32_t ph = 1;
-            for (int t = first; t < tiles; t += pairs) {
+            for (int t = first; t < items; t += pairs) {
                 int nt, kt;
-                tile_of(t, p, nt, kt);
-                const int n0 = nt * kRows + rank * 128;
-                for (int i = 0; i < p.steps; ++i) {
+                tile_of(t / splits, p, nt, kt);
+                const int n0 = nt * kRows + rank * 128, to = to_step(t);
+                for (int i = from_step(t); i < to; ++i) {
                     wait(done(s), ph);
                     __syncwarp();
                     if (elect_one()) {
@@ -218,14 +236,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint64_t desc0 = sw128_matrix(sbase, kPlaneBytes / 2);
             int s = 0, buf = 0;
             uint32_t ph = 0, reuse = 1;
-            for (int t = 0; t < mine; ++t) {
-                for (int i = 0; i < p.steps; ++i) {
+            for (int t = first; t < items; t += pairs) {
+                const int steps = to_step(t) - from_step(t);
+                for (int i = 0; i < steps; ++i) {
                     const int in = i % L::SPAN;
                     if (in == 0) wait(sums_empty(buf), reuse);
                     wait(full(s), ph);
                     __syncwarp();
                     tc_after();
-                    const bool last = in == L::SPAN - 1 || i == p.steps - 1;
+                    const bool last = in == L::SPAN - 1 || i == steps - 1;
                     if (elect_one()) {
                         const uint64_t d0 = desc0 + (uint64_t)(s * (L::STAGE >> 4));
                         const uint64_t dx = d0 + (uint64_t)(P * (kPlaneBytes >> 4));
@@ -254,7 +273,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t full0 = in_cta(full(0), 0);
             int s = 0;
             uint32_t ph = 0;
-            for (int64_t i = (int64_t)mine * p.steps; i > 0; --i) {
+            for (int64_t i = total; i > 0; --i) {
                 wait(made(s), ph);
                 __syncwarp();
                 if (lane == 0) arrive_in_cluster(full0 + 8u * (uint32_t)s);
@@ -268,12 +287,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // and the scales of the block that they lie in
             int a = 0;
             uint32_t ph = 1;
-            for (int t = first; t < tiles; t += pairs) {
+            for (int t = first; t < items; t += pairs) {
                 int nt, kt;
-                tile_of(t, p, nt, kt);
-                const int k0 = kt * TK + rank * (TK / 2);
+                tile_of(t / splits, p, nt, kt);
+                const int k0 = kt * TK + rank * (TK / 2), to = to_step(t);
                 const float* sc = p.scales + (min(k0, p.K - 1) >> 7) * p.s_col;
-                for (int i = 0; i < p.steps; ++i) {
+                for (int i = from_step(t); i < to; ++i) {
                     wait(codes_read(a), ph);
                     __syncwarp();
                     if (elect_one()) {
@@ -314,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes);
         int s = turn, a = turn;
         uint32_t ph = 1, aph = 0;
-        for (int64_t left = ((int64_t)mine * p.steps + 1 - turn) >> 1; left > 0; --left) {
+        for (int64_t left = (total + 1 - turn) >> 1; left > 0; --left) {
             uint2 code[4][2];         // eight codes of each 64 columns
             float scale[4];
             if (!try_wait_both(codes_full(a), aph, done(s), ph)) {
@@ -378,11 +397,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t free0 = in_cta(sums_empty(0), 0);
         int buf = 0;
         uint32_t ph = 0;
-        for (int t = first; t < tiles; t += pairs) {
+        for (int t = first; t < items; t += pairs) {
             float acc[TK / 2];
 #pragma unroll
             for (int c = 0; c < TK / 2; ++c) acc[c] = 0.0f;
-            for (int i = 0; i < p.steps; i += L::SPAN) {
+            for (int left = to_step(t) - from_step(t); left > 0; left -= L::SPAN) {
                 wait(sums_full(buf), ph);
                 __syncwarp();
                 tc_after();
@@ -403,11 +422,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 buf ^= 1;
                 if (buf == 0) ph ^= 1u;
             }
+            bool write = true;
+            if constexpr (SPLIT) {
+                // the part's sums go to its slot, [column / 4][row][4]
+                constexpr int64_t SLOT = 128 * TK;
+                const int64_t lane_at = ((int64_t)half * (TK / 8) * 128 + q * 32 + lane) * 4;
+                float4* mine = reinterpret_cast<float4*>(p.part + ((int64_t)t * 2 + rank) * SLOT + lane_at);
+#pragma unroll
+                for (int c = 0; c < TK / 8; ++c)
+                    mine[c * 128] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+                __threadfence();
+                named_barrier(1, 256);
+                volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
+                const int tile = t / splits;
+                if (warp == 12 && lane == 0)
+                    *flag = atomicAdd(p.arrived + tile * 2 + rank, 1u) == (unsigned)(splits - 1);
+                named_barrier(1, 256);
+                write = *flag != 0u;
+                named_barrier(1, 256);   // the flag has been read
+                if (write) {
+                    __threadfence();
+#pragma unroll
+                    for (int c = 0; c < TK / 2; ++c) acc[c] = 0.0f;
+#pragma unroll 1
+                    for (int sp = 0; sp < splits; ++sp) {
+                        const float4* src = reinterpret_cast<const float4*>(
+                            p.part + (((int64_t)tile * splits + sp) * 2 + rank) * SLOT + lane_at);
+#pragma unroll
+                        for (int c = 0; c < TK / 8; ++c) {
+                            const float4 f = __ldcg(src + c * 128);
+                            acc[4 * c] += f.x;
+                            acc[4 * c + 1] += f.y;
+                            acc[4 * c + 2] += f.z;
+                            acc[4 * c + 3] += f.w;
+                        }
+                    }
+                }
+            }
             int nt, kt;
-            tile_of(t, p, nt, kt);
+            tile_of(t / splits, p, nt, kt);
             const int64_t n = (int64_t)nt * kRows + rank * 128 + q * 32 + lane;
             const int64_t k0 = (int64_t)kt * TK + half * (TK / 2);
-            if (n < p.N) {
+            if (write && n < p.N) {
 #pragma unroll
                 for (int c = 0; c < TK / 2; c += 16) {
                     float v[16];
@@ -427,14 +483,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // dy as bf16 terms that add up to it (fp16: 2, fp32: 3), each [M, ld] below the
 // last: v cut off to bf16, then what is left (cut off, no term overflows and eight
-// bits go into each). A value that is not finite has it
-// in the first term and zeros below. bf16 input whose rows TMA cannot read (an odd
-// stride or address) is copied as its one term.
+// bits go into each). A value that is not finite has it in the first term and zeros
+// below. bf16 input whose rows TMA cannot read (an odd stride or address) is copied as
+// its one term. The product's counters are zeroed on the way.
 template <typename T, int P>
 __global__ void __launch_bounds__(256) split_terms_kernel(const T* __restrict__ dy, int64_t M, int64_t N, int64_t ldy,
-                                                          __nv_bfloat16* __restrict__ out, int64_t ld) {
+                                                          __nv_bfloat16* __restrict__ out, int64_t ld, unsigned int* arrived,
+                                                          int64_t n_arrived) {
     grid_wait();
     launch_dependents();
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n_arrived;
+         i += (int64_t)gridDim.x * blockDim.x)
+        arrived[i] = 0u;
     const int64_t quads = ld / 4;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < M * quads;
          i += (int64_t)gridDim.x * blockDim.x) {
@@ -467,8 +527,62 @@ int terms_of(int type) { return type == kBf16 ? 1 : (type == kF16 ? 2 : 3); }
 int64_t term_ld(int64_t N) { return (N + 7) / 8 * 8; }
 int bytes_of(int type) { return type == kF32 ? 4 : 2; }
 
-template <int P, int TK, typename O>
-cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
+constexpr int64_t kMostSplits = 16;
+
+bool rows_by_tma(const void* dy, int type, int64_t ldy) {
+    return type == kBf16 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0 && (ldy * 2) % 16 == 0;
+}
+size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
+
+// The tile's columns and the parts that its rows are cut into: the shortest by a model
+// in microseconds, fitted at 512 to 8192 rows of 128 x 128 to 11008 x 4096: the rounds
+// of steps over the pairs of SMs, a wide step taking 0.45 with one term, 0.65 with two
+// and 0.92 with three, a narrow one 0.6 of that; parts cost 7 and 0.5 for each, for
+// their sums written and read by the last pair to arrive. Without and with parts:
+// 8192 x 128 x 128 (bf16 dy) 37 / 22, (fp32 dy) 62 / 22; 65536 x 256 x 256 260 / 39;
+// 4096 x 768 x 768 22 / 21; 1024 x 512 x 512 (9.4) has none.
+struct Plan {
+    int tk, splits;
+};
+Plan plan_of(int64_t M, int64_t N, int64_t K, int dy_type) {
+    const int64_t pairs = sm_count() / 2, rows = (N + kRows - 1) / kRows, steps = (M + kStep - 1) / kStep;
+    const int terms = terms_of(dy_type);
+    const double wide_us = terms == 1 ? 0.45 : (terms == 2 ? 0.65 : 0.92), narrow_us = 0.6 * wide_us;
+    const int64_t wide = rows * ((K + 255) / 256), narrow = rows * ((K + 127) / 128);
+    double best = wide_us * (double)((wide + pairs - 1) / pairs * steps);
+    Plan plan{256, 1};
+    const double one = narrow_us * (double)((narrow + pairs - 1) / pairs * steps);
+    if (one < best) {
+        best = one;
+        plan = Plan{128, 1};
+    }
+    int64_t most = pairs / narrow;
+    if (most > steps / 4) most = steps / 4;
+    if (most > kMostSplits) most = kMostSplits;
+    for (int64_t n = 2; n <= most; ++n) {
+        const double us = narrow_us * (double)((steps + n - 1) / n) + 7.0 + 0.5 * (double)n;
+        if (us < best) {
+            best = us;
+            plan = Plan{128, (int)n};
+        }
+    }
+    return plan;
+}
+// The workspace: terms of dy (where they are needed), the counters, the parts' sums.
+size_t terms_bytes(int64_t M, int64_t N, int type) {
+    return round_up((size_t)terms_of(type) * (size_t)M * (size_t)term_ld(N) * 2);
+}
+int64_t plan_tiles(int64_t N, int64_t K, int tk) { return (N + kRows - 1) / kRows * ((K + tk - 1) / tk); }
+size_t arrived_bytes(const Plan& plan, int64_t N, int64_t K) {
+    return plan.splits == 1 ? 0 : round_up((size_t)plan_tiles(N, K, plan.tk) * 2 * 4);
+}
+size_t part_bytes(const Plan& plan, int64_t N, int64_t K) {
+    return plan.splits == 1 ? 0 : (size_t)plan_tiles(N, K, plan.tk) * plan.splits * 2 * 128 * plan.tk * 4;
+}
+
+template <int P, int TK, bool SPLIT, typename O>
+cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, int splits, unsigned char* counters,
+                      cudaStream_t s) {
     Params p;
     p.scales = g.a.scales;
     p.s_row = g.a.s_row;
@@ -488,6 +602,9 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
     const int64_t bands = (p.tiles_k + band - 1) / band;
     p.band = (int)((p.tiles_k + bands - 1) / bands);
     p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * bytes_of(g.out_type)) % 32 == 0;
+    p.splits = splits;
+    p.arrived = SPLIT ? reinterpret_cast<unsigned int*>(counters) : nullptr;
+    p.part = SPLIT ? reinterpret_cast<float*>(counters + arrived_bytes(Plan{TK, splits}, g.N, g.K)) : nullptr;
     p.fault = fault_word();
     if (p.fault == nullptr) return cudaErrorInvalidDevicePointer;
     CUtensorMap map, mx;
@@ -495,49 +612,53 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaSt
         !encode_codes(&mx, g.a.codes, g.a.cols, g.a.rows, g.a.ld, kStep))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)Smem<P, TK>::TOTAL + 1024;
-    auto kern = fp8_wgrad_kernel<P, TK, O>;
+    auto kern = fp8_wgrad_kernel<P, TK, SPLIT, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kLaunchRegs, ready);
     if (e != cudaSuccess) return e;
-    const int tiles = p.tiles_n * p.tiles_k;
-    const int pairs = sm_count() / 2;
-    LaunchConfig cfg(dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), kThreads, smem, s);
+    const int64_t items = (int64_t)p.tiles_n * p.tiles_k * splits;
+    const int64_t pairs = sm_count() / 2;
+    if (items > 0x7fffffff) return cudaErrorInvalidValue;
+    LaunchConfig cfg(dim3(2u * (unsigned)(items < pairs ? items : pairs)), kThreads, smem, s);
     return cudaLaunchKernelEx(&cfg.c, kern, p, map, mx);
 }
 
 template <int P, typename O>
-cudaError_t launch_tile(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
-    // rounds of tiles over the pairs of SMs, times a tile's time: 128 columns take
-    // 0.6 of what 256 do
-    const int64_t pairs = sm_count() / 2, rows = (g.N + kRows - 1) / kRows;
-    const int64_t wide = (rows * ((g.K + 255) / 256) + pairs - 1) / pairs;
-    const int64_t narrow = (rows * ((g.K + 127) / 128) + pairs - 1) / pairs;
-    return 10 * wide <= 6 * narrow ? launch_po<P, 256, O>(g, dy, ld, s) : launch_po<P, 128, O>(g, dy, ld, s);
+cudaError_t launch_tile(const Fp8WeightGrad& g, const void* dy, int64_t ld, const Plan& plan, unsigned char* counters,
+                        cudaStream_t s) {
+    if (plan.splits > 1) return launch_po<P, 128, true, O>(g, dy, ld, plan.splits, counters, s);
+    return plan.tk == 256 ? launch_po<P, 256, false, O>(g, dy, ld, 1, nullptr, s)
+                          : launch_po<P, 128, false, O>(g, dy, ld, 1, nullptr, s);
 }
 
 template <int P>
-cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, cudaStream_t s) {
-    if (g.out_type == kF16) return launch_tile<P, __half>(g, dy, ld, s);
-    if (g.out_type == kBf16) return launch_tile<P, __nv_bfloat16>(g, dy, ld, s);
-    return launch_tile<P, float>(g, dy, ld, s);
+cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, const Plan& plan, unsigned char* counters,
+                     cudaStream_t s) {
+    if (g.out_type == kF16) return launch_tile<P, __half>(g, dy, ld, plan, counters, s);
+    if (g.out_type == kBf16) return launch_tile<P, __nv_bfloat16>(g, dy, ld, plan, counters, s);
+    return launch_tile<P, float>(g, dy, ld, plan, counters, s);
 }
 
 template <typename T, int P>
-cudaError_t split_and_launch(const Fp8WeightGrad& g, void* workspace, cudaStream_t s) {
+cudaError_t split_and_launch(const Fp8WeightGrad& g, void* workspace, const Plan& plan, cudaStream_t s) {
     const int64_t ld = term_ld(g.N);
     const int64_t want = (g.M * (ld / 4) + 255) / 256;
     const int64_t most = (int64_t)sm_count() * 16;
+    unsigned char* counters = static_cast<unsigned char*>(workspace) + terms_bytes(g.M, g.N, g.dy_type);
     LaunchConfig cfg(dim3((unsigned)(want < most ? want : most)), 256, 0, s);
     cudaError_t e = cudaLaunchKernelEx(&cfg.c, split_terms_kernel<T, P>, static_cast<const T*>(g.dy), g.M, g.N, g.ldy,
-                                       static_cast<__nv_bfloat16*>(workspace), ld);
+                                       static_cast<__nv_bfloat16*>(workspace), ld,
+                                       reinterpret_cast<unsigned int*>(counters),
+                                       (int64_t)(arrived_bytes(plan, g.N, g.K) / 4));
     if (e != cudaSuccess) return e;
-    return launch_p<P>(g, workspace, ld, s);
+    return launch_p<P>(g, workspace, ld, plan, counters, s);
 }
 
 }  // namespace
 
-size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t, int dy_type) {
-    return (size_t)terms_of(dy_type) * (size_t)M * (size_t)term_ld(N) * 2;
+size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type) {
+    const Plan plan = plan_of(M, N, K, dy_type);
+    return terms_bytes(M, N, dy_type) + arrived_bytes(plan, N, K) + part_bytes(plan, N, K);
 }
 
 cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cudaStream_t s) {
@@ -551,11 +672,16 @@ cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cuda
         else zero_rows_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(g.out), g.N, g.K, g.ldo);
         return cudaGetLastError();
     }
-    if (g.dy_type == kF32) return split_and_launch<float, 3>(g, workspace, s);
-    if (g.dy_type == kF16) return split_and_launch<__half, 2>(g, workspace, s);
-    if ((reinterpret_cast<uintptr_t>(g.dy) & 15) != 0 || (g.ldy * 2) % 16 != 0)
-        return split_and_launch<__nv_bfloat16, 1>(g, workspace, s);
-    return launch_p<1>(g, g.dy, g.ldy, s);
+    const Plan plan = plan_of(g.M, g.N, g.K, g.dy_type);
+    if (g.dy_type == kF32) return split_and_launch<float, 3>(g, workspace, plan, s);
+    if (g.dy_type == kF16) return split_and_launch<__half, 2>(g, workspace, plan, s);
+    if (!rows_by_tma(g.dy, g.dy_type, g.ldy)) return split_and_launch<__nv_bfloat16, 1>(g, workspace, plan, s);
+    unsigned char* counters = static_cast<unsigned char*>(workspace) + terms_bytes(g.M, g.N, g.dy_type);
+    if (plan.splits > 1) {
+        cudaError_t e = cudaMemsetAsync(counters, 0, arrived_bytes(plan, g.N, g.K), s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_p<1>(g, g.dy, g.ldy, plan, counters, s);
 }
 
 }  // namespace wq
