@@ -110,6 +110,19 @@ __device__ __forceinline__ void tile_of(int t, const PairParams& p, int& mt, int
 // store that ends at y's edges and drains while the next tile's blocks are summed:
 // stores from registers held the tile's hand-off for 4300 cycles, every CTA's 64 KB
 // at once.
+template <typename O>
+__device__ __forceinline__ O ld_shared(uint32_t at) {
+    if constexpr (sizeof(O) == 4) {
+        uint32_t v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return *reinterpret_cast<const O*>(&v);
+    } else {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+        return *reinterpret_cast<const O*>(&v);
+    }
+}
+
 template <typename O, int C>
 __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap* map, uint32_t out, int lane,
                                          int64_t m0, int64_t n0, const uint64_t (&acc)[C / 2]) {
@@ -122,35 +135,44 @@ __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap*
         if (has_bias && n0 + c < p.N) v += load_any(p.bias, p.bias_type, n0 + c);
         return from_f32<O>(v);
     };
-    if (p.tma_out) {
 #pragma unroll
-        for (int c0 = 0; c0 < C; c0 += BOX) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
+    for (int c0 = 0; c0 < C; c0 += BOX) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                uint32_t w[4];
-                O e[PER];
+        for (int k = 0; k < 8; ++k) {
+            uint32_t w[4];
+            O e[PER];
 #pragma unroll
-                for (int j = 0; j < PER; ++j) e[j] = value(c0 + k * PER + j);
+            for (int j = 0; j < PER; ++j) e[j] = value(c0 + k * PER + j);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint32_t*>(e)[j];
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((k ^ (lane & 7)) << 4)),
-                             "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                             : "memory");
-            }
+            for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint32_t*>(e)[j];
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((k ^ (lane & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+        if (p.tma_out) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 if (m0 < p.M && n0 + c0 < p.N) tma_store(map, (int)(n0 + c0), (int)m0, out);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-        }
-    } else if (m0 + lane < p.M) {
-        O* row = static_cast<O*>(p.out) + (m0 + lane) * p.ldo + n0;
+        } else {
+            // rows that TMA cannot write: a row's neighbouring columns by the warp
+            __syncwarp();
+            const int rows = (int)(p.M - m0 < 32 ? p.M - m0 : 32);
+            O* at = static_cast<O*>(p.out) + m0 * p.ldo + n0 + c0 + lane;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, at += p.ldo) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (n0 + c < p.N) row[c] = value(c);
+                for (int h = 0; h < BOX; h += 32) {
+                    const int c = h + lane;
+                    const O v = ld_shared<O>(out + r * 128 + (((c / PER) ^ (r & 7)) << 4) + c % PER * (int)sizeof(O));
+                    if (n0 + c0 + c < p.N) at[h] = v;
+                }
+            }
+        }
     }
 }
 
