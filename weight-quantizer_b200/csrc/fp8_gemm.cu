@@ -105,11 +105,6 @@ __device__ __forceinline__ void tile_of(int t, const PairParams& p, int& mt, int
     mt = b * p.band + (in - nt * bw);
 }
 
-// A warp's 32 rows (from m0) x C columns (from n0) of y out of its sums: a lane is
-// a row. By way of shared memory (128 bytes of 32 rows at a time, swizzled) and a TMA
-// store that ends at y's edges and drains while the next tile's blocks are summed:
-// stores from registers held the tile's hand-off for 4300 cycles, every CTA's 64 KB
-// at once.
 template <typename O>
 __device__ __forceinline__ O ld_shared(uint32_t at) {
     if constexpr (sizeof(O) == 4) {
@@ -123,6 +118,11 @@ __device__ __forceinline__ O ld_shared(uint32_t at) {
     }
 }
 
+// A warp's 32 rows (from m0) x C columns (from n0) of y out of its sums: a lane is
+// a row. By way of shared memory (128 bytes of 32 rows at a time, swizzled) and a TMA
+// store that ends at y's edges and drains while the next tile's blocks are summed:
+// stores from registers held the tile's hand-off for 4300 cycles, every CTA's 64 KB
+// at once.
 template <typename O, int C>
 __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap* map, uint32_t out, int lane,
                                          int64_t m0, int64_t n0, const uint64_t (&acc)[C / 2]) {
@@ -135,10 +135,7 @@ __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap*
         if (has_bias && n0 + c < p.N) v += load_any(p.bias, p.bias_type, n0 + c);
         return from_f32<O>(v);
     };
-#pragma unroll
-    for (int c0 = 0; c0 < C; c0 += BOX) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
+    auto stage = [&](int c0) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             uint32_t w[4];
@@ -151,17 +148,29 @@ __device__ __forceinline__ void put_tile(const PairParams& p, const CUtensorMap*
                          "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                          : "memory");
         }
-        if (p.tma_out) {
+    };
+    if (p.tma_out) {
+#pragma unroll
+        for (int c0 = 0; c0 < C; c0 += BOX) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+            stage(c0);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 if (m0 < p.M && n0 + c0 < p.N) tma_store(map, (int)(n0 + c0), (int)m0, out);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-        } else {
-            // rows that TMA cannot write: a row's neighbouring columns by the warp
+        }
+    } else {
+        // rows that TMA cannot write: a row's neighbouring columns by the warp (single
+        // elements of 32 rows per store took 416 us at 4096 x 11007 x 256, these 48)
+        const int rows = (int)(p.M - m0 < 32 ? p.M - m0 : 32);
+#pragma unroll
+        for (int c0 = 0; c0 < C; c0 += BOX) {
             __syncwarp();
-            const int rows = (int)(p.M - m0 < 32 ? p.M - m0 : 32);
+            stage(c0);
+            __syncwarp();
             O* at = static_cast<O*>(p.out) + m0 * p.ldo + n0 + c0 + lane;
 #pragma unroll 8
             for (int r = 0; r < rows; ++r, at += p.ldo) {

@@ -94,35 +94,34 @@ __device__ __forceinline__ void tile_of(int t, const Params& p, int& nt, int& kt
     kt = b * p.band + (in - nt * bw);
 }
 
-// Columns c .. c + 15 of 32 rows of dw, a lane's own row in v. Rows that lie 32 bytes
-// apart are written as they are. Others go through a transposition inside the warp
-// (bits of the lane change places with bits of the register), after which a lane has
-// one column of 16 rows and a store fills 16 neighbouring columns: single elements of
-// 32 rows per store took 752 us at 16 x 14336 x 8191 (fp32).
+// Columns c .. c + 15 of a row of dw whose rows lie 32 bytes apart.
 template <typename O>
-__device__ __forceinline__ void put16(const Params& p, int64_t n0, int lane, int64_t c, float (&v)[16]) {
-    O* out = static_cast<O*>(p.out);
-    const bool add = p.accumulate != 0;
-    if (p.wide_out && c + 16 <= p.K) {
-        if (n0 + lane >= p.N) return;
-        O* row = out + (n0 + lane) * p.ldo;
-        constexpr int PER = 4 / (int)sizeof(O);       // values in a word
+__device__ __forceinline__ void put16(O* at, const float (&v)[16], bool add) {
+    constexpr int PER = 4 / (int)sizeof(O);       // values in a word
 #pragma unroll
-        for (int i = 0; i < 16; i += 8 * PER) {
-            uint32_t w[8];
+    for (int i = 0; i < 16; i += 8 * PER) {
+        uint32_t w[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                O e[PER];
-                if (add) *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(row + c + i + q * PER);
+        for (int q = 0; q < 8; ++q) {
+            O e[PER];
+            if (add) *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(at + i + q * PER);
 #pragma unroll
-                for (int j = 0; j < PER; ++j)
-                    e[j] = from_f32<O>(add ? to_f32<O>(e[j]) + v[i + q * PER + j] : v[i + q * PER + j]);
-                w[q] = *reinterpret_cast<const uint32_t*>(e);
-            }
-            st_32(row + c + i, w);
+            for (int j = 0; j < PER; ++j)
+                e[j] = from_f32<O>(add ? to_f32<O>(e[j]) + v[i + q * PER + j] : v[i + q * PER + j]);
+            w[q] = *reinterpret_cast<const uint32_t*>(e);
         }
-        return;
+        st_32(at + i, w);
     }
+}
+
+// The same 16 columns of a warp's 32 rows where rows lie otherwise, or end inside: a
+// transposition inside the warp (bits of the lane change places with bits of the
+// register), after which a lane has one column of 16 rows and a store fills 16
+// neighbouring columns. Single elements of 32 rows per store took 752 us at
+// 16 x 14336 x 8191 (fp32), these 216.
+template <typename O>
+__device__ __forceinline__ void put16_across(O* out, int64_t n0, int64_t c, int64_t rows, int64_t cols, int64_t ld,
+                                             int lane, float (&v)[16], bool add) {
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) {
         const bool up = (lane & d) != 0;
@@ -135,12 +134,12 @@ __device__ __forceinline__ void put16(const Params& p, int64_t n0, int lane, int
         }
     }
     const int64_t col = c + (lane & 15), n = n0 + (lane & 16);
-    if (col >= p.K) return;
-    O* at = out + n * p.ldo + col;
+    if (col >= cols) return;
+    O* at = out + n * ld + col;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (n + i < p.N) {
-            O* e = at + i * p.ldo;
+        if (n + i < rows) {
+            O* e = at + i * ld;
             *e = from_f32<O>(add ? to_f32<O>(*e) + v[i] : v[i]);
         }
 }
@@ -488,13 +487,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tile_of(t / splits, p, nt, kt);
             const int64_t n0 = (int64_t)nt * kRows + rank * 128 + q * 32;
             const int64_t k0 = (int64_t)kt * TK + half * (TK / 2);
-            if (write && n0 < p.N) {
+            O* out = static_cast<O*>(p.out);
+            if (p.wide_out && k0 + TK / 2 <= p.K) {
+                if (write && n0 + lane < p.N) {
+#pragma unroll
+                    for (int c = 0; c < TK / 2; c += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
+                        put16<O>(out + (n0 + lane) * p.ldo + k0 + c, v, p.accumulate);
+                    }
+                }
+            } else if (write && n0 < p.N) {
 #pragma unroll
                 for (int c = 0; c < TK / 2; c += 16) {
                     float v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
-                    if (k0 + c < p.K) put16<O>(p, n0, lane, k0 + c, v);
+                    if (k0 + c < p.K) put16_across<O>(out, n0, k0 + c, p.N, p.K, p.ldo, lane, v, p.accumulate);
                 }
             }
         }
