@@ -77,7 +77,6 @@ struct Params {
     int accumulate;
     int M, N, K, steps;
     int tiles_n, tiles_k, band;
-    bool wide_out;
     int splits;              // parts of the rows
     float* part;             // [tile][part][rank] sums of 128 x TK
     unsigned int* arrived;   // per tile and rank, zeroed before the launch
@@ -144,7 +143,9 @@ __device__ __forceinline__ void put16_across(O* out, int64_t n0, int64_t c, int6
         }
 }
 
-template <int P, int TK, bool SPLIT, typename O>
+// WIDE: rows of dw lie 32 bytes apart and K is a multiple of 16. (A kernel of its own: both
+// ways in one cost registers: 1.4% at 8192 x 11008 x 4096.)
+template <int P, int TK, bool SPLIT, bool WIDE, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const Params p, const __grid_constant__ CUtensorMap map_dy,
                      const __grid_constant__ CUtensorMap map_x) {
@@ -488,23 +489,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int64_t n0 = (int64_t)nt * kRows + rank * 128 + q * 32;
             const int64_t k0 = (int64_t)kt * TK + half * (TK / 2);
             O* out = static_cast<O*>(p.out);
-            if (p.wide_out && k0 + TK / 2 <= p.K) {
-                if (write && n0 + lane < p.N) {
-#pragma unroll
-                    for (int c = 0; c < TK / 2; c += 16) {
-                        float v[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
-                        put16<O>(out + (n0 + lane) * p.ldo + k0 + c, v, p.accumulate);
-                    }
-                }
-            } else if (write && n0 < p.N) {
+            if (WIDE ? write && n0 + lane < p.N : write && n0 < p.N) {
 #pragma unroll
                 for (int c = 0; c < TK / 2; c += 16) {
                     float v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
-                    if (k0 + c < p.K) put16_across<O>(out, n0, k0 + c, p.N, p.K, p.ldo, lane, v, p.accumulate);
+                    if (k0 + c < p.K) {
+                        if constexpr (WIDE) put16<O>(out + (n0 + lane) * p.ldo + k0 + c, v, p.accumulate);
+                        else put16_across<O>(out, n0, k0 + c, p.N, p.K, p.ldo, lane, v, p.accumulate);
+                    }
                 }
             }
         }
@@ -567,6 +561,9 @@ constexpr int64_t kMostSplits = 16;
 bool rows_by_tma(const void* dy, int type, int64_t ldy) {
     return type == kBf16 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0 && (ldy * 2) % 16 == 0;
 }
+bool wide_rows(const Fp8WeightGrad& g) {
+    return (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * bytes_of(g.out_type)) % 32 == 0 && g.K % 16 == 0;
+}
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 
 // The tile's columns and the parts that its rows are cut into: the shortest by a model
@@ -615,7 +612,7 @@ size_t part_bytes(const Plan& plan, int64_t N, int64_t K) {
     return plan.splits == 1 ? 0 : (size_t)plan_tiles(N, K, plan.tk) * plan.splits * 2 * 128 * plan.tk * 4;
 }
 
-template <int P, int TK, bool SPLIT, typename O>
+template <int P, int TK, bool SPLIT, bool WIDE, typename O>
 cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, int splits, unsigned char* counters,
                       cudaStream_t s) {
     Params p;
@@ -636,7 +633,6 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, int sp
     band = band < 1 ? 1 : band;
     const int64_t bands = (p.tiles_k + band - 1) / band;
     p.band = (int)((p.tiles_k + bands - 1) / bands);
-    p.wide_out = (reinterpret_cast<uintptr_t>(g.out) & 31) == 0 && (g.ldo * bytes_of(g.out_type)) % 32 == 0;
     p.splits = splits;
     p.arrived = SPLIT ? reinterpret_cast<unsigned int*>(counters) : nullptr;
     p.part = SPLIT ? reinterpret_cast<float*>(counters + arrived_bytes(Plan{TK, splits}, g.N, g.K)) : nullptr;
@@ -647,7 +643,7 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, int sp
         !encode_codes(&mx, g.a.codes, g.a.cols, g.a.rows, g.a.ld, kStep))
         return cudaErrorInvalidValue;
     const size_t smem = (size_t)Smem<P, TK>::TOTAL + 1024;
-    auto kern = fp8_wgrad_kernel<P, TK, SPLIT, O>;
+    auto kern = fp8_wgrad_kernel<P, TK, SPLIT, WIDE, O>;
     static std::atomic<int> ready[kMaxDevices];
     cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, kLaunchRegs, ready);
     if (e != cudaSuccess) return e;
@@ -661,9 +657,13 @@ cudaError_t launch_po(const Fp8WeightGrad& g, const void* dy, int64_t ld, int sp
 template <int P, typename O>
 cudaError_t launch_tile(const Fp8WeightGrad& g, const void* dy, int64_t ld, const Plan& plan, unsigned char* counters,
                         cudaStream_t s) {
-    if (plan.splits > 1) return launch_po<P, 128, true, O>(g, dy, ld, plan.splits, counters, s);
-    return plan.tk == 256 ? launch_po<P, 256, false, O>(g, dy, ld, 1, nullptr, s)
-                          : launch_po<P, 128, false, O>(g, dy, ld, 1, nullptr, s);
+    // (parts make few tiles: one way of writing them serves)
+    if (plan.splits > 1) return launch_po<P, 128, true, false, O>(g, dy, ld, plan.splits, counters, s);
+    if (wide_rows(g))
+        return plan.tk == 256 ? launch_po<P, 256, false, true, O>(g, dy, ld, 1, nullptr, s)
+                              : launch_po<P, 128, false, true, O>(g, dy, ld, 1, nullptr, s);
+    return plan.tk == 256 ? launch_po<P, 256, false, false, O>(g, dy, ld, 1, nullptr, s)
+                          : launch_po<P, 128, false, false, O>(g, dy, ld, 1, nullptr, s);
 }
 
 template <int P>
