@@ -60,11 +60,13 @@ struct Smem {
     static constexpr int CODES = STAGES * STAGE;
     static constexpr int SCALES = CODES + kAhead * kCodesBytes;
     static constexpr int BAR = SCALES + kAhead * kStep * 4;
-    // full and done per stage; the odd CTA's x^ ready per stage; codes there and read;
-    // sums full[2], empty[2]
-    static constexpr int TMEM_SLOT = BAR + 8 * (3 * STAGES + 2 * kAhead + 4);
+    // full and done per stage; codes there and read; sums full[2], empty[2]
+    static constexpr int TMEM_SLOT = BAR + 8 * (2 * STAGES + 2 * kAhead + 4);
     static constexpr int FLAG = TMEM_SLOT + 8;
-    static constexpr int TOTAL = TMEM_SLOT + 16;
+    // a token to send, and where tokens go: one for each warp that makes a stage's x^
+    static constexpr int TOKEN = TMEM_SLOT + 16;
+    static constexpr int TOTAL = TOKEN + 16 * (1 + 4 * STAGES);
+    static_assert(TOKEN % 16 == 0, "bulk copies are 16-byte aligned");
     static_assert(STAGES >= 2, "the MMAs of one step run while the next is made");
     static_assert(TOTAL + 1024 <= 227 * 1024, "stages exceed the shared memory of one CTA");
 };
@@ -160,19 +162,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto bar = [&](int i) -> uint32_t { return sbase + L::BAR + 8u * (uint32_t)i; };
     auto full = [&](int s) { return bar(s); };
     auto done = [&](int s) { return bar(NS + s); };
-    auto made = [&](int s) { return bar(2 * NS + s); };
-    auto codes_full = [&](int a) { return bar(3 * NS + a); };
-    auto codes_read = [&](int a) { return bar(3 * NS + kAhead + a); };
-    auto sums_full = [&](int b) { return bar(3 * NS + 2 * kAhead + b); };
-    auto sums_empty = [&](int b) { return bar(3 * NS + 2 * kAhead + 2 + b); };
+    auto codes_full = [&](int a) { return bar(2 * NS + a); };
+    auto codes_read = [&](int a) { return bar(2 * NS + kAhead + a); };
+    auto sums_full = [&](int b) { return bar(2 * NS + 2 * kAhead + b); };
+    auto sums_empty = [&](int b) { return bar(2 * NS + 2 * kAhead + 2 + b); };
     launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            // the even CTA's: its loader's arrival with both CTAs' bytes of dy, its four
-            // warps that made x^, and one word that the odd CTA's x^ is there
-            mbar_init(full(s), 6);
+            // the even CTA's: its loader's arrival with both CTAs' bytes of dy and the
+            // tokens of the odd CTA's four warps that made x^, and its own four
+            mbar_init(full(s), 5);
             mbar_init(done(s), 1);
-            mbar_init(made(s), 4);
         }
         for (int a = 0; a < kAhead; ++a) {
             mbar_init(codes_full(a), 33);   // the codes' bytes, and every lane's copies of scales
@@ -183,6 +183,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(sums_empty(b), 16);
         }
         fence_mbarrier_init();
+        *reinterpret_cast<uint4*>(smem + L::TOKEN) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
     }
     if (warp == 1) tmem_alloc<2>(sbase + L::TMEM_SLOT, 512);
     tc_before();
@@ -207,11 +209,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     else
         total = first < items ? (int64_t)((items - 1 - first) / pairs + 1) * p.steps : 0;
     bool faulted = false;
+    auto give_up = [&]() {
+        faulted = true;
+        atomicOr(p.fault, 1u);
+    };
     auto wait = [&](uint32_t b, uint32_t parity) {
-        if (!faulted && !mbar_wait_bounded(b, parity)) {
-            faulted = true;
-            atomicOr(p.fault, 1u);
-        }
+        if (!faulted && !mbar_wait_bounded(b, parity)) give_up();
     };
 
     if (warp < 4) {
@@ -230,7 +233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (elect_one()) {
                         const uint32_t f = full0 + 8u * (uint32_t)s;
                         const uint32_t dst = sbase + (uint32_t)(s * L::STAGE);
-                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * P * kPlaneBytes);
+                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * P * kPlaneBytes + 4 * 16);
 #pragma unroll
                         for (int pl = 0; pl < P; ++pl) {
                             // term pl of dy lies pl * M rows below the first; the rows
@@ -266,7 +269,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < steps; ++i) {
                     const int in = i % L::SPAN;
                     if (in == 0) wait(sums_empty(buf), reuse);
-                    wait(full(s), ph);
+                    // acquires the odd CTA's x^ too, which its warps' tokens release
+                    if (!faulted && !mbar_wait_cluster(full(s), ph)) give_up();
                     __syncwarp();
                     tc_after();
                     const bool last = in == L::SPAN - 1 || i == steps - 1;
@@ -291,20 +295,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         s = 0;
                         ph ^= 1u;
                     }
-                }
-            }
-        } else if (warp == 2 && rank == 1) {
-            // passes the odd CTA's finished x^ on to the even CTA's barrier
-            const uint32_t full0 = in_cta(full(0), 0);
-            int s = 0;
-            uint32_t ph = 0;
-            for (int64_t i = total; i > 0; --i) {
-                wait(made(s), ph);
-                __syncwarp();
-                if (lane == 0) arrive_in_cluster(full0 + 8u * (uint32_t)s);
-                if (++s == NS) {
-                    s = 0;
-                    ph ^= 1u;
                 }
             }
         } else if (warp == 3) {
@@ -356,6 +346,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int row0 = q * 16 + (sub >> 1) + 4 * (sub & 1);
         auto row_of = [&](int j) { return row0 + 2 * (j & 1) + 8 * (j >> 1); };
         const uint32_t x_at = sbase + (uint32_t)(P * kPlaneBytes);
+        const uint32_t full0 = in_cta(full(0), 0), tokens0 = in_cta(sbase + L::TOKEN + 16u, 0) + 16u * (uint32_t)q;
         int s = turn, a = turn;
         uint32_t ph = 1, aph = 0;
         for (int64_t left = (total + 1 - turn) >> 1; left > 0; --left) {
@@ -401,7 +392,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(rank == 0 ? full(s) : made(s));
+                if (rank == 0) mbar_arrive(full(s));
+                else token_to_cta(tokens0 + 64u * (uint32_t)s, sbase + L::TOKEN, full0 + 8u * (uint32_t)s);
                 mbar_arrive(codes_read(a));
             }
             a += 2;
