@@ -401,6 +401,14 @@ WQ_API int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N,
                               int64_t K, int64_t ld, const float* scales, int64_t s_row, int64_t s_col, void* dw,
                               int dw_type, int64_t ldw, int accumulate, void* workspace, size_t workspace_bytes,
                               void* stream);
+/* The kernel that sizes take on the current device, for tests and measurements. A   */
+/* product: WQ_FP8_FEW_ROWS with the rows of a that its tile holds (16, 32 or 64), or */
+/* WQ_FP8_PAIRS with the tile's columns of out (128 or 256) and the parts that the    */
+/* inner dimension is cut into. A weight gradient (always pairs): the tile's columns  */
+/* of dw and the parts that the rows are cut into. Sizes of at least 1.              */
+enum wq_fp8_kernel { WQ_FP8_PAIRS = 0, WQ_FP8_FEW_ROWS = 1 };
+WQ_API int wq_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int* kernel, int* tile, int* parts);
+WQ_API int wq_fp8_weight_grad_plan(int64_t M, int64_t N, int64_t K, int dy_type, int* tile, int* parts);
 /* out [cols] = the sum of x [rows, cols] over its rows, in fp32, rounded once:  */
 /* the layer's bias gradient.                                                   */
 WQ_API int wq_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out,

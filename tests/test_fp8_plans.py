@@ -1,0 +1,33 @@
+"""Which kernel of the 8-bit floating-point operators sizes take, asked without a GPU (148 SMs are assumed then):
+the sizes of test_fp8_paths_gpu.py take the kernels that they are there to test, and every kernel has some."""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from test_fp8_paths_gpu import GRADIENTS, PRODUCTS
+
+
+def test_sizes_take_the_kernels_they_test(wq) -> None:
+    for size, plan in PRODUCTS.items():
+        assert wq._kernels.fp8_gemm_plan(*size) == plan, size
+    kinds = {(k, t, p > 1) for k, t, p in PRODUCTS.values()}
+    assert kinds == {("few rows", t, False) for t in (16, 32, 64)} | {("pairs", t, p) for t in (128, 256)
+                                                                     for p in (False, True)}
+    for size, plan in GRADIENTS.items():
+        for dtype in (torch.bfloat16, torch.float16, torch.float32):
+            assert wq._kernels.fp8_weight_grad_plan(*size, dtype) == plan, size
+
+
+def test_plan_c_refusals(wq) -> None:
+    lib = wq._kernels.library()
+    a, b, c = (ctypes.c_int() for _ in range(3))
+    p = lib.wq_fp8_gemm_plan
+    assert p(0, 8, 8, a, b, c) == 5 and p(8, -1, 8, a, b, c) == 5
+    assert p(1 << 23, 8, 8, a, b, c) == 13
+    assert p(8, 8, 8, None, b, c) == 11 and p(8, 8, 8, a, b, c) == 0
+    g = lib.wq_fp8_weight_grad_plan
+    assert g(8, 8, 0, 0, a, b) == 5 and g(8, 8, 8, 3, a, b) == 23 and g(8, 8, 8, 0, None, b) == 11
+    assert g(8, 8, 1 << 23, 0, a, b) == 13 and g(8, 8, 8, 2, a, b) == 0

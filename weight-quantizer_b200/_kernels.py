@@ -29,6 +29,7 @@ _ARG_ERRORS_AS_VALUEERROR = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 15, 16, 
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_pint = ctypes.POINTER(ctypes.c_int)
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 
@@ -103,6 +104,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _int,
         [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _i64, _int, _vp, _sz, _vp],
     ),
+    "wq_fp8_gemm_plan": (_int, [_i64, _i64, _i64, _pint, _pint, _pint]),
+    "wq_fp8_weight_grad_plan": (_int, [_i64, _i64, _i64, _int, _pint, _pint]),
     "wq_column_sum": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _vp]),
 }
 
@@ -872,6 +875,21 @@ def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
               (dy.data_ptr(), dy_type, M, N, ldy, codes.data_ptr(), K, ld, scales.data_ptr(), *scales.stride(),
                dw.data_ptr(), out_type, ldw, int(accumulate), None if ws is None else ws.data_ptr(), nws), True)
     return dw
+
+
+def fp8_gemm_plan(M: int, N: int, K: int) -> tuple[str, int, int]:
+    """The kernel that a product of these sizes takes on the current device: ("few rows", rows of a that its tile
+    holds, 1) or ("pairs", the tile's columns, parts of the inner dimension)."""
+    kernel, tile, parts = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    _check(library().wq_fp8_gemm_plan(M, N, K, ctypes.byref(kernel), ctypes.byref(tile), ctypes.byref(parts)))
+    return ("few rows" if kernel.value == 1 else "pairs"), tile.value, parts.value
+
+
+def fp8_weight_grad_plan(M: int, N: int, K: int, dtype: torch.dtype) -> tuple[int, int]:
+    """(columns of dw in a tile, parts of the rows) for a weight gradient from dy of ``dtype``."""
+    tile, parts = ctypes.c_int(), ctypes.c_int()
+    _check(library().wq_fp8_weight_grad_plan(M, N, K, _dtype(dtype, "dtype"), ctypes.byref(tile), ctypes.byref(parts)))
+    return tile.value, parts.value
 
 
 def column_sum(x: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:

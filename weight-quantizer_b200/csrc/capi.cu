@@ -723,6 +723,33 @@ int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_
     return e == cudaSuccess ? WQ_OK : cuda_fail(e);
 }
 
+static int fp8_plan_args(int64_t M, int64_t N, int64_t K) {
+    if (M < 1 || N < 1 || K < 1) return WQ_E_NEG_DIM;
+    return M > kMaxFp8Rows || N > kMaxFp8Cols || K > kMaxFp8Cols ? WQ_E_TOO_LARGE : WQ_OK;
+}
+
+int wq_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int* kernel, int* tile, int* parts) {
+    if (kernel == nullptr || tile == nullptr || parts == nullptr) return WQ_E_NULL;
+    const int bad = fp8_plan_args(M, N, K);
+    if (bad != WQ_OK) return bad;
+    const wq::Fp8Plan plan = wq::fp8_gemm_plan(M, N, K);
+    *kernel = plan.few_rows ? WQ_FP8_FEW_ROWS : WQ_FP8_PAIRS;
+    *tile = plan.tile;
+    *parts = plan.parts;
+    return WQ_OK;
+}
+
+int wq_fp8_weight_grad_plan(int64_t M, int64_t N, int64_t K, int dy_type, int* tile, int* parts) {
+    if (tile == nullptr || parts == nullptr) return WQ_E_NULL;
+    if (!fp8_type_ok(dy_type)) return WQ_E_DTYPE;
+    const int bad = fp8_plan_args(M, N, K);
+    if (bad != WQ_OK) return bad;
+    const wq::Fp8Plan plan = wq::fp8_weight_grad_plan(M, N, K, dy_type);
+    *tile = plan.tile;
+    *parts = plan.parts;
+    return WQ_OK;
+}
+
 int wq_column_sum(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, void* out, int out_type,
                   void* stream) {
     if (!fp8_type_ok(x_type) || !fp8_type_ok(out_type)) return WQ_E_DTYPE;

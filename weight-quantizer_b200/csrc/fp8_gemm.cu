@@ -1026,6 +1026,12 @@ size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     return pair_plan(M, N, K).splits > 1 ? pair_arrived_bytes(M, N, K) + pair_part_bytes(M, N, K) : 0;
 }
 
+Fp8Plan fp8_gemm_plan(int64_t M, int64_t N, int64_t K) {
+    if (few_rows(M, N, K)) return Fp8Plan{true, few_width(M), 1};
+    const PairPlan plan = pair_plan(M, N, K);
+    return Fp8Plan{false, plan.tn, plan.splits};
+}
+
 cudaError_t launch_fp8_gemm(const Fp8Gemm& g, void* workspace, bool prepared, cudaStream_t s) {
     if (g.K == 0) {
         const int64_t n = (g.M * g.N + 255) / 256;

@@ -688,6 +688,11 @@ size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_t
     return terms_bytes(M, N, dy_type) + arrived_bytes(plan, N, K) + part_bytes(plan, N, K);
 }
 
+Fp8Plan fp8_weight_grad_plan(int64_t M, int64_t N, int64_t K, int dy_type) {
+    const Plan plan = plan_of(M, N, K, dy_type);
+    return Fp8Plan{false, plan.tk, plan.splits};
+}
+
 cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cudaStream_t s) {
     if (g.M == 0) {
         if (g.accumulate) return cudaSuccess;

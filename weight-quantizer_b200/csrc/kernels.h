@@ -194,6 +194,14 @@ struct Fp8WeightGrad {
     int accumulate;   // add to out's values
 };
 size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type);
+// The kernel that sizes take: `tile` rows of a (few rows) or columns of the output,
+// `parts` of the sum.
+struct Fp8Plan {
+    bool few_rows;
+    int tile, parts;
+};
+Fp8Plan fp8_gemm_plan(int64_t M, int64_t N, int64_t K);
+Fp8Plan fp8_weight_grad_plan(int64_t M, int64_t N, int64_t K, int dy_type);
 cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cudaStream_t s);
 
 // Number of SMs of the current device (cached per device).
