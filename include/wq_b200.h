@@ -396,7 +396,13 @@ WQ_API int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_
 /* [M, N] has row stride ldy. Scales that are powers of two (wq_fp8_quantize's) */
 /* make x^ exact in bf16, the product's operand type; with other scales x^ is   */
 /* rounded to bf16. accumulate != 0 adds to dw's values.                        */
+/* Workspace: a dy that the kernel cannot read as it is goes there as bf16 terms: */
+/* fp32 as three (1.5 times dy's bytes), fp16 as two, bf16 only where dy or its    */
+/* row stride is not a multiple of 16 bytes. _for says what a given dy needs,      */
+/* _bytes what every dy of the type can do with.                                   */
 WQ_API size_t wq_fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type);
+WQ_API size_t wq_fp8_weight_grad_workspace_for(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy,
+                                               int64_t K);
 WQ_API int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy, const uint8_t* codes,
                               int64_t K, int64_t ld, const float* scales, int64_t s_row, int64_t s_col, void* dw,
                               int dw_type, int64_t ldw, int accumulate, void* workspace, size_t workspace_bytes,

@@ -1,0 +1,57 @@
+"""The 8-bit floating-point layer in a model: conversion, freezing, devices, mixed precision, memory."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_fp8_gpu import check_product, rand, values64
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- memory --------------------------------------------------------------------------------
+
+
+def test_weight_grad_of_bf16_keeps_no_copy_of_dy(wq, cuda) -> None:
+    """dy in bf16 whose rows TMA reads is read where it is: beside dw the call holds no more than the parts' sums
+    (here none); other dy is copied, fp16 and fp32 as two and three bf16 terms."""
+    M, N, K = 4096, 4096, 512
+    x = wq.quantize_fp8(rand((M, K), 1, torch.bfloat16))
+    dw = torch.empty(N, K, device=cuda)
+
+    def held(dy: torch.Tensor) -> int:
+        wq.fp8_weight_grad(dy, x, out=dw)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        wq.fp8_weight_grad(dy, x, out=dw)
+        return torch.cuda.max_memory_allocated() - before
+
+    assert wq._kernels.fp8_weight_grad_plan(M, N, K, torch.bfloat16)[1] == 1
+    dy = rand((M, N), 2, torch.bfloat16, 1e-2)
+    assert held(dy) == 0
+    check_product(dw, dy.double().t(), values64(x))
+    wide = torch.zeros(M, N + 3, dtype=torch.bfloat16, device=cuda)
+    wide[:, 3:] = dy
+    assert held(wide[:, 3:]) == M * N * 2     # rows that TMA cannot read
+    check_product(dw, dy.double().t(), values64(x))
+    for dtype, terms in ((torch.float16, 2), (torch.float32, 3)):
+        d2 = rand((M, N), 2, dtype, 1e-2)
+        assert held(d2) == M * N * 2 * terms
+        check_product(dw, d2.double().t(), values64(x))
+
+
+@pytest.mark.parametrize("M,N,K", [(8192, 128, 128), (4100, 304, 520)])
+def test_weight_grad_in_parts_reads_bf16_where_it_is(wq, cuda, M: int, N: int, K: int) -> None:
+    """The counters and sums of parts lie where the terms would begin: right with aligned and other rows, in turn."""
+    assert wq._kernels.fp8_weight_grad_plan(M, N, K, torch.bfloat16)[1] > 1
+    x = wq.quantize_fp8(rand((M, K), 2, torch.bfloat16))
+    dy = rand((M, N), 1, torch.bfloat16, 1e-2)
+    odd = torch.zeros(M, N + 1, dtype=torch.bfloat16, device=cuda)
+    odd[:, 1:] = dy
+    want = wq.fp8_weight_grad(dy, x)
+    check_product(want, dy.double().t(), values64(x))
+    for _ in range(5):
+        assert torch.equal(wq.fp8_weight_grad(odd[:, 1:], x), want)
+        assert torch.equal(wq.fp8_weight_grad(dy, x), want)

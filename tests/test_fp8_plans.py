@@ -31,3 +31,30 @@ def test_plan_c_refusals(wq) -> None:
     g = lib.wq_fp8_weight_grad_plan
     assert g(8, 8, 0, 0, a, b) == 5 and g(8, 8, 8, 3, a, b) == 23 and g(8, 8, 8, 0, None, b) == 11
     assert g(8, 8, 1 << 23, 0, a, b) == 13 and g(8, 8, 8, 2, a, b) == 0
+
+
+def test_weight_grad_workspace(wq) -> None:
+    """bf16 rows that TMA reads need no terms; the query by type covers every dy of the type."""
+    lib = wq._kernels.library()
+    M, N, K = 8192, 28672, 4096
+    assert wq._kernels.fp8_weight_grad_plan(M, N, K, torch.bfloat16)[1] == 1
+    every, this = lib.wq_fp8_weight_grad_workspace_bytes, lib.wq_fp8_weight_grad_workspace_for
+    at = ctypes.c_void_p
+    assert this(at(256), 2, M, N, N, K) == 0
+    for dy, ld in ((258, N), (256, N + 1)):
+        assert this(at(dy), 2, M, N, ld, K) == M * N * 2 == every(M, N, K, 2)
+    assert this(at(256), 1, M, N, N, K) == M * N * 2 * 2 == every(M, N, K, 1)
+    assert this(at(256), 0, M, N, N, K) == M * N * 2 * 3 == every(M, N, K, 0)
+    # in parts: the counters and sums, with or without the terms
+    assert wq._kernels.fp8_weight_grad_plan(8192, 128, 128, torch.bfloat16)[1] > 1
+    parts = this(at(256), 2, 8192, 128, 128, 128)
+    assert parts > 0 and this(at(256), 2, 8192, 128, 129, 128) == parts + 8192 * 128 * 2
+    assert this(at(256), 2, 0, N, N, K) == 0
+    # the call asks for what its dy needs
+    p, big = at(256), 1 << 40
+
+    def call(dy, ld, ws, nws):  # type: ignore[no-untyped-def]
+        return lib.wq_fp8_weight_grad(dy, 2, M, N, ld, p, K, K, p, 1, M, p, 0, K, 0, ws, nws, None)
+
+    assert call(at(258), N, None, 0) == 12 and call(p, N + 1, p, M * N * 2 - 1) == 12
+    assert call(at(258), N, at(128), big) == 12

@@ -100,6 +100,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
          _vp, _int, _i64, _vp, _sz, _vp],
     ),
     "wq_fp8_weight_grad_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "wq_fp8_weight_grad_workspace_for": (_sz, [_vp, _int, _i64, _i64, _i64, _i64]),
     "wq_fp8_weight_grad": (
         _int,
         [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _i64, _int, _vp, _sz, _vp],
@@ -869,7 +870,7 @@ def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     dy, ldy = _rows(dy)
     codes, ld = _codes_arg(codes)
     lib = library()
-    nws = lib.wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type)
+    nws = lib.wq_fp8_weight_grad_workspace_for(dy.data_ptr(), dy_type, M, N, ldy, K)
     ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev) if nws else None
     _fp8_call(lib.wq_fp8_weight_grad, dev,
               (dy.data_ptr(), dy_type, M, N, ldy, codes.data_ptr(), K, ld, scales.data_ptr(), *scales.stride(),

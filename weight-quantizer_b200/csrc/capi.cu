@@ -700,7 +700,12 @@ int wq_fp8_linear(const void* x, int x_type, int64_t M, int64_t K, int64_t ldx, 
 }
 
 size_t wq_fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type) {
-    return M <= 0 || N <= 0 || K <= 0 ? 0 : wq::fp8_weight_grad_workspace_bytes(M, N, K, dy_type);
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : wq::fp8_weight_grad_workspace_bytes(M, N, K, dy_type, true);
+}
+
+size_t wq_fp8_weight_grad_workspace_for(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return wq::fp8_weight_grad_workspace_bytes(M, N, K, dy_type, !wq::fp8_weight_grad_reads(dy, dy_type, ldy));
 }
 
 int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_t ldy, const uint8_t* codes, int64_t K,
@@ -715,7 +720,7 @@ int wq_fp8_weight_grad(const void* dy, int dy_type, int64_t M, int64_t N, int64_
     if (N == 0 || K == 0) return WQ_OK;
     if (dw == nullptr) return WQ_E_NULL;
     if (M > 0 && (dy == nullptr || codes == nullptr || scales == nullptr)) return WQ_E_NULL;
-    const size_t need = wq_fp8_weight_grad_workspace_bytes(M, N, K, dy_type);
+    const size_t need = wq_fp8_weight_grad_workspace_for(dy, dy_type, M, N, ldy, K);
     if (!fp8_workspace_ok(workspace, workspace_bytes, need)) return WQ_E_WORKSPACE;
     const wq::Fp8Operand ao{codes, M, K, ld, scales, s_row, s_col, 1};
     const wq::Fp8WeightGrad g{dy, dy_type, ldy, ao, M, N, K, dw, dw_type, ldw, accumulate ? 1 : 0};

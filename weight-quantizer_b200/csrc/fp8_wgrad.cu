@@ -592,7 +592,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int dy_type) {
     }
     return plan;
 }
-// The workspace: terms of dy (where they are needed), the counters, the parts' sums.
+// The workspace: the counters and the parts' sums where there are parts, then the terms of
+// dy where dy is not read as it is.
 size_t terms_bytes(int64_t M, int64_t N, int type) {
     return round_up((size_t)terms_of(type) * (size_t)M * (size_t)term_ld(N) * 2);
 }
@@ -667,25 +668,27 @@ cudaError_t launch_p(const Fp8WeightGrad& g, const void* dy, int64_t ld, const P
 }
 
 template <typename T, int P>
-cudaError_t split_and_launch(const Fp8WeightGrad& g, void* workspace, const Plan& plan, cudaStream_t s) {
+cudaError_t split_and_launch(const Fp8WeightGrad& g, unsigned char* counters, const Plan& plan, cudaStream_t s) {
     const int64_t ld = term_ld(g.N);
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(counters + arrived_bytes(plan, g.N, g.K) +
+                                                            part_bytes(plan, g.N, g.K));
     const int64_t want = (g.M * (ld / 4) + 255) / 256;
     const int64_t most = (int64_t)sm_count() * 16;
-    unsigned char* counters = static_cast<unsigned char*>(workspace) + terms_bytes(g.M, g.N, g.dy_type);
     LaunchConfig cfg(dim3((unsigned)(want < most ? want : most)), 256, 0, s);
     cudaError_t e = cudaLaunchKernelEx(&cfg.c, split_terms_kernel<T, P>, static_cast<const T*>(g.dy), g.M, g.N, g.ldy,
-                                       static_cast<__nv_bfloat16*>(workspace), ld,
-                                       reinterpret_cast<unsigned int*>(counters),
+                                       terms, ld, reinterpret_cast<unsigned int*>(counters),
                                        (int64_t)(arrived_bytes(plan, g.N, g.K) / 4));
     if (e != cudaSuccess) return e;
-    return launch_p<P>(g, workspace, ld, plan, counters, s);
+    return launch_p<P>(g, terms, ld, plan, counters, s);
 }
 
 }  // namespace
 
-size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type) {
+bool fp8_weight_grad_reads(const void* dy, int dy_type, int64_t ldy) { return rows_by_tma(dy, dy_type, ldy); }
+
+size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type, bool terms) {
     const Plan plan = plan_of(M, N, K, dy_type);
-    return terms_bytes(M, N, dy_type) + arrived_bytes(plan, N, K) + part_bytes(plan, N, K);
+    return arrived_bytes(plan, N, K) + part_bytes(plan, N, K) + (terms ? terms_bytes(M, N, dy_type) : 0);
 }
 
 Fp8Plan fp8_weight_grad_plan(int64_t M, int64_t N, int64_t K, int dy_type) {
@@ -705,10 +708,10 @@ cudaError_t launch_fp8_weight_grad(const Fp8WeightGrad& g, void* workspace, cuda
         return cudaGetLastError();
     }
     const Plan plan = plan_of(g.M, g.N, g.K, g.dy_type);
-    if (g.dy_type == kF32) return split_and_launch<float, 3>(g, workspace, plan, s);
-    if (g.dy_type == kF16) return split_and_launch<__half, 2>(g, workspace, plan, s);
-    if (!rows_by_tma(g.dy, g.dy_type, g.ldy)) return split_and_launch<__nv_bfloat16, 1>(g, workspace, plan, s);
-    unsigned char* counters = static_cast<unsigned char*>(workspace) + terms_bytes(g.M, g.N, g.dy_type);
+    unsigned char* counters = static_cast<unsigned char*>(workspace);
+    if (g.dy_type == kF32) return split_and_launch<float, 3>(g, counters, plan, s);
+    if (g.dy_type == kF16) return split_and_launch<__half, 2>(g, counters, plan, s);
+    if (!rows_by_tma(g.dy, g.dy_type, g.ldy)) return split_and_launch<__nv_bfloat16, 1>(g, counters, plan, s);
     if (plan.splits > 1) {
         cudaError_t e = cudaMemsetAsync(counters, 0, arrived_bytes(plan, g.N, g.K), s);
         if (e != cudaSuccess) return e;

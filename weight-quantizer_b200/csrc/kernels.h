@@ -193,7 +193,10 @@ struct Fp8WeightGrad {
     int64_t ldo;
     int accumulate;   // add to out's values
 };
-size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type);
+// Whether the kernel reads dy where it is (bf16 rows that TMA can read); other dy is
+// written to the workspace as its bf16 terms.
+bool fp8_weight_grad_reads(const void* dy, int dy_type, int64_t ldy);
+size_t fp8_weight_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dy_type, bool terms);
 // The kernel that sizes take: `tile` rows of a (few rows) or columns of the output,
 // `parts` of the sum.
 struct Fp8Plan {
