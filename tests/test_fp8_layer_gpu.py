@@ -4,10 +4,38 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch import nn
 
 from test_fp8_gpu import check_product, rand, values64
 
 pytestmark = pytest.mark.gpu
+
+
+def net(cuda) -> nn.Module:  # type: ignore[no-untyped-def]
+    torch.manual_seed(0)
+    return nn.Sequential(nn.Linear(200, 333), nn.ReLU(), nn.Linear(333, 130)).to(cuda)
+
+
+# ---- freezing ------------------------------------------------------------------------
+
+
+def test_freezing_a_converted_model(wq, cuda) -> None:
+    """Convert, train a step, convert again with freeze: every layer keeps its 8-bit tiles alone and answers as it
+    did."""
+    model = wq.fp8_model(net(cuda))
+    x = rand((20, 200), 1)
+    model(x).sum().backward()
+    with torch.no_grad():
+        want = model(x)
+        assert wq.fp8_model(model, freeze=True) is model
+        layers = [m for m in model.modules() if isinstance(m, wq.Fp8Linear)]
+        assert len(layers) == 2 and all(m.weight is None and m.codes is not None for m in layers)
+        assert torch.equal(model(x), want)
+    one = wq.Fp8Linear(rand((64, 200), 2))
+    assert wq.fp8_model(one, freeze=True) is one and one.weight is None
+    mixed = nn.Sequential(wq.Fp8Linear(rand((64, 200), 2)), nn.Linear(64, 32, device=cuda))
+    wq.fp8_model(mixed, freeze=True)
+    assert all(isinstance(m, wq.Fp8Linear) and m.weight is None for m in mixed)
 
 
 # ---- memory --------------------------------------------------------------------------------

@@ -267,7 +267,8 @@ def quantize_model(
 def fp8_model(model: nn.Module, *, freeze: bool = False) -> nn.Module:
     """Replace every nn.Linear and Conv1D of ``model`` in place by an ``Fp8Linear`` over
     the same weight and bias: 8-bit operands in both directions, 8-bit checkpoints of
-    the layers' inputs. ``freeze`` keeps the weights as 8-bit tiles only, for serving.
+    the layers' inputs. ``freeze`` keeps the weights as 8-bit tiles only, for serving, and
+    does so for the ``Fp8Linear`` layers that are there already, a converted model's.
     A model that is itself the only target comes back as the replacement layer. An
     nn.Linear's parameters stay the same objects (ties and optimizers keep them); a
     Conv1D's weight is transposed into a new parameter. No ptqkit counterpart."""
@@ -287,4 +288,8 @@ def fp8_model(model: nn.Module, *, freeze: bool = False) -> nn.Module:
             root = layer
         else:
             _set_module(model, name, layer)
+    if freeze:
+        for m in root.modules():
+            if isinstance(m, Fp8Linear):
+                m.freeze()
     return root
