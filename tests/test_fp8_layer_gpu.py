@@ -38,6 +38,18 @@ def test_freezing_a_converted_model(wq, cuda) -> None:
     assert all(isinstance(m, wq.Fp8Linear) and m.weight is None for m in mixed)
 
 
+# ---- shared modules ------------------------------------------------------------------
+
+
+def test_a_module_under_two_names(wq, cuda) -> None:
+    """A layer that the model holds twice is replaced in both places, by one layer."""
+    model = nn.Module()
+    model.first = nn.Linear(64, 64, device=cuda)
+    model.inner = nn.Sequential(nn.ReLU(), model.first)
+    wq.fp8_model(model)
+    assert isinstance(model.first, wq.Fp8Linear) and model.inner[1] is model.first
+
+
 # ---- memory --------------------------------------------------------------------------------
 
 

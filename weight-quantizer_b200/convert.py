@@ -275,7 +275,10 @@ def fp8_model(model: nn.Module, *, freeze: bool = False) -> nn.Module:
     if any(p.device.type != "cuda" for p in model.parameters()):
         raise RuntimeError("fp8_model expects CUDA parameters")
     root: nn.Module = model
-    for name, module in iter_targets(model):
+    names: dict[nn.Module, list[str]] = {}   # a module may be held under several
+    for name, module in model.named_modules(remove_duplicate=False):
+        names.setdefault(module, []).append(name)
+    for _, module in iter_targets(model):
         if isinstance(module, nn.Linear):
             layer = Fp8Linear.from_linear(module)
         else:
@@ -284,10 +287,11 @@ def fp8_model(model: nn.Module, *, freeze: bool = False) -> nn.Module:
         layer.train(module.training)
         if freeze:
             layer.freeze()
-        if name == "":
-            root = layer
-        else:
-            _set_module(model, name, layer)
+        for name in names[module]:
+            if name == "":
+                root = layer
+            else:
+                _set_module(model, name, layer)
     if freeze:
         for m in root.modules():
             if isinstance(m, Fp8Linear):
