@@ -2,11 +2,13 @@
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 from torch import nn
 
-from test_fp8_gpu import check_product, rand, values64
+from test_fp8_gpu import E4M3, check_product, rand, values64
 
 pytestmark = pytest.mark.gpu
 
@@ -48,6 +50,39 @@ def test_a_module_under_two_names(wq, cuda) -> None:
     model.inner = nn.Sequential(nn.ReLU(), model.first)
     wq.fp8_model(model)
     assert isinstance(model.first, wq.Fp8Linear) and model.inner[1] is model.first
+
+
+# ---- a frozen layer's rows -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("move", ["device", "copy", "assign", "operand"])
+def test_moved_codes_keep_rows_that_the_products_read(wq, cuda, move: str) -> None:
+    """A width that is no multiple of 16: after a way over the host, or a load that takes the state's tensors as they
+    are, the codes lie in padded rows again, and a product allocates no copy of them."""
+    layer = wq.Fp8Linear(rand((4096, 1001), 1, torch.bfloat16, 0.02)).freeze()
+    x = rand((4, 1001), 2, torch.bfloat16)
+    want = layer(x)
+    if move == "device":
+        layer = layer.cpu().to(cuda)
+    elif move == "copy":
+        layer = copy.deepcopy(layer)
+    elif move == "assign":
+        state = {k: v.contiguous() if v.dtype != E4M3 else v.view(torch.uint8).contiguous().view(E4M3)
+                 for k, v in layer.state_dict().items()}
+        assert state["codes"].stride(0) == 1001
+        layer.load_state_dict(state, assign=True)
+    else:
+        q = layer.quantized_weight().to("cpu").to(cuda)
+        assert torch.equal(wq.fp8_gemm(x, q), want)
+        layer.codes = q.codes
+    assert layer.codes.shape == (4096, 1001) and layer.codes.stride(0) % 16 == 0
+    layer(x)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = layer(x)
+    assert torch.equal(y, want)
+    assert torch.cuda.max_memory_allocated() - before < 4096 * 1001
 
 
 # ---- memory --------------------------------------------------------------------------------

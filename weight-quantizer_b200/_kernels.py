@@ -763,6 +763,15 @@ def _codes_arg(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
     return kept, pitch
 
 
+def fp8_padded(codes: torch.Tensor) -> torch.Tensor:
+    """``codes`` as the products read them without a copy at each call: themselves, or a copy in padded rows (a device
+    copy or a contiguous load has lost the padding). On the host they stay as they are."""
+    if not codes.is_cuda:
+        return codes
+    kept, _ = _codes_arg(codes)
+    return codes if kept is codes else kept.view(codes.dtype)[:, : codes.shape[1]]
+
+
 def _empty(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
     """A dense matrix (torch.empty takes half again as long as the strided form)."""
     return torch.empty_strided((rows, cols), (cols if cols > 0 else 1, 1), dtype=dtype, device=dev)

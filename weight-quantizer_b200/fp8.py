@@ -68,8 +68,8 @@ class Fp8Blocks:
         return int(self.codes.shape[0]), int(self.codes.shape[1])
 
     def to(self, device: torch.device | str) -> Fp8Blocks:
-        """Copy of this operand with both tensors on ``device``."""
-        return Fp8Blocks(self.codes.to(device), self.scales.to(device), self.block_rows)
+        """Copy of this operand with both tensors on ``device`` (codes in padded rows on a GPU)."""
+        return Fp8Blocks(_kernels.fp8_padded(self.codes.to(device)), self.scales.to(device), self.block_rows)
 
 
 def _flat(x: torch.Tensor) -> torch.Tensor:
@@ -253,13 +253,19 @@ class Fp8Linear(nn.Module):
         return self
 
     def _apply(self, fn: Callable[..., Any], recurse: bool = True) -> Fp8Linear:
-        # a cast (half(), to(dtype)) is for the parameters: codes and scales only move
+        # a cast (half(), to(dtype)) is for the parameters: codes and scales only move, and
+        # a copy of rows that do not fill their pitch comes without the padding
         codes, scales = self.codes, self.scales
         super()._apply(fn, recurse=recurse)  # type: ignore[no-untyped-call]
         if codes is not None and scales is not None and self.scales is not None:
             dev = self.scales.device
-            self.codes, self.scales = codes.to(dev), scales.to(dev)
+            self.codes, self.scales = _kernels.fp8_padded(codes.to(dev)), scales.to(dev)
         return self
+
+    def _load_from_state_dict(self, *args: Any, **kwargs: Any) -> None:
+        super()._load_from_state_dict(*args, **kwargs)  # type: ignore[no-untyped-call]
+        if self.codes is not None:   # (with assign=True the state's own tensors)
+            self.codes = _kernels.fp8_padded(self.codes)
 
     def quantized_weight(self) -> Fp8Blocks:
         """The weight as the products read it."""
