@@ -85,6 +85,43 @@ def test_moved_codes_keep_rows_that_the_products_read(wq, cuda, move: str) -> No
     assert torch.cuda.max_memory_allocated() - before < 4096 * 1001
 
 
+# ---- mixed precision ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast(wq, cuda, dtype) -> None:
+    """Under autocast the layer takes and gives autocast's type, as nn.Linear does, and its fp32 weight is quantized
+    as it is; gradients come in their parameters' types."""
+    plain = net(cuda)
+    model = wq.fp8_model(copy.deepcopy(plain))
+    x = rand((20, 200), 1)
+    with torch.autocast("cuda", dtype=dtype):
+        assert plain(x).dtype == dtype
+        y = model(x)
+        assert y.dtype == dtype
+    w = model[0].weight
+    h = wq.fp8_linear(x.to(dtype), w, model[0].bias)
+    with torch.autocast("cuda", dtype=dtype):
+        assert torch.equal(wq.fp8_linear(x, w, model[0].bias), h)
+        assert wq.fp8_linear(x.double().float(), w).dtype == dtype
+    check_product(h.detach(), values64(wq.quantize_fp8(x.to(dtype))), values64(wq.quantize_fp8(w, block_rows=128)).t(),
+                  model[0].bias)
+    xg = x.clone().requires_grad_()
+    with torch.autocast("cuda", dtype=dtype):
+        y = wq.fp8_linear(xg, w)
+    dy = rand(y.shape, 3, dtype, 1e-2)
+    dx, dw = torch.autograd.grad(y, (xg, w), dy)
+    assert dx.dtype == dw.dtype == torch.float32
+    check_product(dw, dy.double().t(), values64(wq.quantize_fp8(x.to(dtype))))
+    assert torch.equal(dx, wq.fp8_gemm(dy, wq.quantize_fp8(w, block_rows=128), transpose=True).float())
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        want = model(x)
+        wq.fp8_model(model, freeze=True)
+        assert torch.equal(model(x), want)
+    with torch.autocast("cuda", dtype=dtype, enabled=False):
+        assert wq.fp8_linear(x, w).dtype == torch.float32
+
+
 # ---- memory --------------------------------------------------------------------------------
 
 

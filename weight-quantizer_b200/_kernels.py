@@ -692,6 +692,9 @@ FP8_BLOCK = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # wq_dtype
 
 
+FP8_INPUTS = frozenset(_DTYPES)
+
+
 def _dtype(t: torch.dtype, what: str) -> int:
     code = _DTYPES.get(t)
     if code is None:

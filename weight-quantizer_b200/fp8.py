@@ -189,12 +189,22 @@ class _Fp8LinearFn(torch.autograd.Function):
         return dx, dw, db
 
 
+def _autocast(x: torch.Tensor) -> torch.Tensor:
+    """x in the type that a linear layer takes it in: under autocast autocast's, otherwise its own."""
+    if torch.is_autocast_enabled("cuda") and x.is_cuda and x.dtype in _kernels.FP8_INPUTS:
+        return x.to(torch.get_autocast_dtype("cuda"))
+    return x
+
+
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight^T + bias`` from 8-bit operands, differentiable (see the module docstring).
 
     ``x`` [..., in], ``weight`` [out, in] and ``bias`` [out] are float32, float16
     or bfloat16; the result has x's type, each gradient its input's. Of ``x`` the
     graph keeps the 8-bit codes and their scales, of ``weight`` its 8-bit tiles.
+    Under ``torch.autocast`` x is cast to autocast's type first, as a linear layer's
+    input is, and the result has that type; weight and bias are read as they are.
+    (``torch.func`` transforms refuse it.)
     """
     if weight.ndim != 2:
         raise ValueError("weight must have shape [out, in]")
@@ -205,7 +215,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     for name, t in (("x", x), ("weight", weight), ("bias", bias)):
         if t is not None and t.device.type != "cuda":
             raise ValueError(f"{name} must be a CUDA tensor")
-    return _Fp8LinearFn.apply(x, weight, bias)
+    return _Fp8LinearFn.apply(_autocast(x), weight, bias)
 
 
 class Fp8Linear(nn.Module):
@@ -281,7 +291,7 @@ class Fp8Linear(nn.Module):
             return fp8_linear(x, self.weight, self.bias)
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("a frozen Fp8Linear has no backward pass; call it under torch.no_grad()")
-        return fp8_gemm(x, self.quantized_weight(), bias=self.bias)
+        return fp8_gemm(_autocast(x), self.quantized_weight(), bias=self.bias)
 
     def extra_repr(self) -> str:
         return (f"in={self.in_features}, out={self.out_features}, block={FP8_BLOCK}, "
