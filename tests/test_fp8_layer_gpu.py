@@ -122,6 +122,12 @@ def test_autocast(wq, cuda, dtype) -> None:
         assert wq.fp8_linear(x, w).dtype == torch.float32
 
 
+def test_func_transforms_are_refused(wq, cuda) -> None:
+    x, w = rand((4, 64), 1), rand((32, 64), 2)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda v: wq.fp8_linear(x, v).sum())(w)
+
+
 # ---- memory --------------------------------------------------------------------------------
 
 

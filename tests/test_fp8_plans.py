@@ -1,5 +1,6 @@
 """Which kernel of the 8-bit floating-point operators sizes take, asked without a GPU (148 SMs are assumed then):
-the sizes of test_fp8_paths_gpu.py take the kernels that they are there to test, and every kernel has some."""
+the sizes of test_fp8_paths_gpu.py take the kernels that they are there to test, and every kernel has some. What a
+call asks of the library, on which device."""
 
 from __future__ import annotations
 
@@ -58,3 +59,56 @@ def test_weight_grad_workspace(wq) -> None:
 
     assert call(at(258), N, None, 0) == 12 and call(p, N + 1, p, M * N * 2 - 1) == 12
     assert call(at(258), N, at(128), big) == 12
+
+
+class _Held:
+    """What the calls ask of a tensor, of one that lies on a device that is not here."""
+
+    is_cuda = True
+
+    def __init__(self, dtype: torch.dtype, *shape: int, device: int = 1) -> None:
+        self.dtype, self.shape, self.ndim = dtype, shape, len(shape)
+        self.device = torch.device("cuda", device)
+
+    def stride(self, i: int | None = None):  # type: ignore[no-untyped-def]
+        s = (self.shape[1], 1)
+        return s if i is None else s[i]
+
+    def numel(self) -> int:
+        return self.shape[0] * self.shape[1]
+
+    def data_ptr(self) -> int:
+        return 4096
+
+
+def test_sizes_are_asked_for_the_operands_device(wq, monkeypatch) -> None:
+    """With operands on a device that is not the current one, workspaces are sized, and kernels launched, with theirs
+    current; the current device is what it was afterwards."""
+    k = wq._kernels
+    now, seen = [0], []
+
+    class Library:
+        def __getattr__(self, name: str):  # type: ignore[no-untyped-def]
+            def call(*args):  # type: ignore[no-untyped-def]
+                seen.append((name, now[0]))
+                return 0
+            return call
+
+    monkeypatch.setattr(k, "library", Library)
+    monkeypatch.setattr(k, "_fault_check", False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: now.__setitem__(0, d if isinstance(d, int) else d.index))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    e4m3, f32, bf16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
+    a, w = _Held(e4m3, 4, 256), _Held(e4m3, 8, 256)
+    out = _Held(bf16, 4, 8)
+    for device in (1, 0):
+        for t in (a, w, out):
+            t.device = torch.device("cuda", device)
+        sa, sw = _Held(f32, 4, 2, device=device), _Held(f32, 1, 2, device=device)
+        k.fp8_gemm(a, sa, w, sw, False, None, bf16, out)
+        k.fp8_gemm(_Held(bf16, 4, 256, device=device), None, w, sw, False, None, bf16, out)
+        k.fp8_weight_grad(_Held(bf16, 4, 8, device=device), a, sa, f32, _Held(f32, 8, 256, device=device), False)
+        assert len(seen) == 6 and {d for _, d in seen} == {device}, seen
+        assert now == [0]
+        seen.clear()

@@ -712,20 +712,26 @@ def _fp8_device(first: torch.Tensor, *others: torch.Tensor) -> torch.device:
     return dev
 
 
-def _fp8_call(fn: Any, dev: torch.device, args: tuple[Any, ...], check_faults: bool = False) -> None:
-    """One entry point on the device's current stream, with that device current for the launch."""
+def _fp8_call(fn: Any, dev: torch.device, args: tuple[Any, ...], size: Any = None, of: tuple[Any, ...] = ()) -> None:
+    """One entry point on the device's current stream, with that device current for the launch and for ``size(*of)``,
+    the bytes of the workspace that the entry point takes last (the kernels that take one report faults)."""
     prev = torch.cuda.current_device()
-    if prev == dev.index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(prev))
-    else:
+    if prev != dev.index:
         torch.cuda.set_device(dev)
-        try:
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-        finally:
+    try:
+        ws = None
+        if size is not None:
+            nws = size(*of)
+            if nws:
+                ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev)
+            args = (*args, None if ws is None else ws.data_ptr(), nws)
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    finally:
+        if prev != dev.index:
             torch.cuda.set_device(prev)
     if status != WQ_OK:
         _check(status)
-    if check_faults and _fault_check and not torch.cuda.is_current_stream_capturing():
+    if size is not None and _fault_check and not torch.cuda.is_current_stream_capturing():
         with torch.cuda.device(dev):
             _raise_on_fault()
 
@@ -851,20 +857,15 @@ def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor | None, w: torch.Tensor, w_
     lib = library()
     weight = (w.data_ptr(), w_rows, w_cols, ldw, w_scales.data_ptr(), *w_scales.stride(), int(transpose), bias_ptr,
               bias_type, y.data_ptr(), out_type, ldo)
-    ws: torch.Tensor | None = None
-    ws_ptr = None
-    nws = (lib.wq_fp8_linear_workspace_bytes if a_scales is None else lib.wq_fp8_gemm_workspace_bytes)(M, N, K)
-    if nws:
-        ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev)
-        ws_ptr = ws.data_ptr()
     if a_scales is None:
         x_type = _dtype(a.dtype, "a")
         a, ldx = _rows(a)
-        _fp8_call(lib.wq_fp8_linear, dev, (a.data_ptr(), x_type, M, K, ldx, *weight, ws_ptr, nws), True)
+        _fp8_call(lib.wq_fp8_linear, dev, (a.data_ptr(), x_type, M, K, ldx, *weight),
+                  lib.wq_fp8_linear_workspace_bytes, (M, N, K))
     else:
         a, lda = _codes_arg(a)
-        _fp8_call(lib.wq_fp8_gemm, dev, (a.data_ptr(), M, K, lda, a_scales.data_ptr(), *a_scales.stride(), *weight,
-                                         ws_ptr, nws), True)
+        _fp8_call(lib.wq_fp8_gemm, dev, (a.data_ptr(), M, K, lda, a_scales.data_ptr(), *a_scales.stride(), *weight),
+                  lib.wq_fp8_gemm_workspace_bytes, (M, N, K))
     return y
 
 
@@ -882,11 +883,10 @@ def fp8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     dy, ldy = _rows(dy)
     codes, ld = _codes_arg(codes)
     lib = library()
-    nws = lib.wq_fp8_weight_grad_workspace_for(dy.data_ptr(), dy_type, M, N, ldy, K)
-    ws = torch.empty_strided((nws,), (1,), dtype=torch.uint8, device=dev) if nws else None
     _fp8_call(lib.wq_fp8_weight_grad, dev,
               (dy.data_ptr(), dy_type, M, N, ldy, codes.data_ptr(), K, ld, scales.data_ptr(), *scales.stride(),
-               dw.data_ptr(), out_type, ldw, int(accumulate), None if ws is None else ws.data_ptr(), nws), True)
+               dw.data_ptr(), out_type, ldw, int(accumulate)),
+              lib.wq_fp8_weight_grad_workspace_for, (dy.data_ptr(), dy_type, M, N, ldy, K))
     return dw
 
 
