@@ -8,7 +8,7 @@ import pytest
 import torch
 from torch import nn
 
-from test_fp8_gpu import E4M3, check_product, rand, values64
+from test_fp8_gpu import DTYPES, E4M3, check_product, rand, values64
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +173,40 @@ def test_weight_grad_in_parts_reads_bf16_where_it_is(wq, cuda, M: int, N: int, K
     for _ in range(5):
         assert torch.equal(wq.fp8_weight_grad(odd[:, 1:], x), want)
         assert torch.equal(wq.fp8_weight_grad(dy, x), want)
+
+
+# ---- one rounding -----------------------------------------------------------------------------
+
+
+def test_dequantize_rounds_once(wq, cuda) -> None:
+    """code * scale for scales that are no powers of two, rounded once to the type: for products that lie just beside
+    the middle of two 16-bit values a rounding to fp32 before would fall on the middle itself."""
+    codes = torch.arange(256, dtype=torch.uint8, device=cuda).view(E4M3)
+    c64 = codes.double()
+    fine = c64.isfinite() & (c64 != 0)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    scales = torch.exp2(torch.rand(4096, generator=g, device=cuda) * 20 - 10)
+    # scales next to those at which a code's value is the middle of two bf16 or fp16 numbers
+    odd = (torch.arange(1024, device=cuda).double() * 2 + 1)
+    near = []
+    for bits in (8, 11):
+        mid = 1 + odd[: 2 ** (bits - 1)] * 2.0 ** -bits
+        for c in (1.125, 1.25, 1.375, 1.5, 1.75):
+            s = (mid / c).float()
+            near += [s, torch.nextafter(s, torch.full_like(s, 9.0)), torch.nextafter(s, torch.zeros_like(s))]
+    scales = torch.cat([scales, *near])
+    q = wq.Fp8Blocks(codes.view(torch.uint8).expand(scales.numel(), 256).contiguous().view(E4M3), scales[:, None].expand(-1, 2).contiguous())
+    exact = c64 * scales.double()[:, None]     # 4 and 24 bits: exact in 64
+    for dtype in DTYPES:
+        got = wq.dequantize_fp8(q, dtype=dtype)[:, fine].double()
+        want = exact[:, fine]
+        # from half a step past the largest number, (2 - eps) 2^e, the nearest is infinity
+        eps = torch.finfo(dtype).eps
+        over = want.abs() >= torch.finfo(dtype).max * (1 + eps / 2 / (2 - eps))
+        assert torch.equal(got.isinf(), over)
+        got, want = got[~over], want[~over]
+        # nearest: no neighbour of the result lies closer to the exact value (a tie may go either way here)
+        up = torch.nextafter(got.to(dtype), torch.full_like(got, float("inf")).to(dtype)).double()
+        down = torch.nextafter(got.to(dtype), torch.full_like(got, -float("inf")).to(dtype)).double()
+        err = (got - want).abs()
+        assert bool((err <= (up - want).abs()).all()) and bool((err <= (down - want).abs()).all()), dtype

@@ -215,20 +215,57 @@ __global__ void __launch_bounds__(256) fp8_tiles_kernel(const T* __restrict__ x,
     if (threadIdx.x == 0) scales[bi * s_row + bj * s_col] = pow2i(e);
 }
 
-// out = code * scale, rounded once to the output type.
+// code * scale (4 and 24 bits) rounded once to T. A scale that is a power of two has an
+// exact product in fp32. Of others the product is cut off, for the 16-bit types, and its
+// last bit set where anything was: that never falls on the middle of two 16-bit values,
+// as a product rounded to fp32 first may.
+template <typename T, bool POWER>
+__device__ __forceinline__ T value_of(float code, float scale) {
+    if (sizeof(T) == 4 || POWER) return from_f32<T>(code * scale);
+    const uint32_t cut = __float_as_uint(__fmul_rz(code, scale));
+    const bool exact = __fmul_rd(code, scale) == __fmul_ru(code, scale);
+    return from_f32<T>(__uint_as_float(exact ? cut : cut | 1u));
+}
+// out = code * scale, rounded once to the output type. vec: four codes are aligned to their
+// 4 bytes, and four values to theirs. 28672 x 8192 to bf16 262 us (2.7 TB/s; scales that are
+// no powers of two 291), to fp32 275 us (4.3 TB/s): index divisions and conversions, not bytes.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_values_kernel(const uint8_t* __restrict__ codes, int64_t rows,
                                                          int64_t cols, int64_t ldc, int block_rows,
                                                          const float* __restrict__ scales, int64_t s_row,
                                                          int64_t s_col, T* __restrict__ out, int64_t ldo,
-                                                         int64_t quads) {
+                                                         int64_t quads, bool vec) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * quads;
          i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / quads, c = (i - r * quads) * 4;
-        const float s = __ldg(scales + (r / block_rows) * s_row + (c / kFp8Block) * s_col);
+        const float s = __ldg(scales + (block_rows == 1 ? r : r / kFp8Block) * s_row + (c / kFp8Block) * s_col);
+        const int n = cols - c < 4 ? (int)(cols - c) : 4;
+        const uint8_t* from = codes + r * ldc + c;
+        T* at = out + r * ldo + c;
+        uint32_t w = 0;
+        if (vec && n == 4) w = __ldg(reinterpret_cast<const uint32_t*>(from));
+        else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (c + k < cols) out[r * ldo + c + k] = from_f32<T>(e4m3x2_values(codes[r * ldc + c + k]).x * s);
+            for (int k = 0; k < 4; ++k)
+                if (k < n) w |= (uint32_t)from[k] << (8 * k);
+        }
+        const float2 lo = e4m3x2_values(w), hi = e4m3x2_values(w >> 16);
+        alignas(16) T v[4];
+        if (sizeof(T) == 4 || (__float_as_uint(s) & 0x7fffffu) == 0) {
+            v[0] = value_of<T, true>(lo.x, s), v[1] = value_of<T, true>(lo.y, s);
+            v[2] = value_of<T, true>(hi.x, s), v[3] = value_of<T, true>(hi.y, s);
+        } else {
+            v[0] = value_of<T, false>(lo.x, s), v[1] = value_of<T, false>(lo.y, s);
+            v[2] = value_of<T, false>(hi.x, s), v[3] = value_of<T, false>(hi.y, s);
+        }
+        if (vec && n == 4) {
+            using Four = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+            *reinterpret_cast<Four*>(at) = *reinterpret_cast<const Four*>(v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < n) at[k] = v[k];
+        }
     }
 }
 
@@ -299,8 +336,10 @@ cudaError_t values_t(const Fp8Operand& a, T* out, int64_t ldo, cudaStream_t s) {
     const int64_t quads = (a.cols + 3) / 4;
     const int64_t want = (a.rows * quads + 255) / 256;
     const int64_t most = (int64_t)sm_count() * 32;
+    const bool vec = (reinterpret_cast<uintptr_t>(a.codes) & 3) == 0 && a.ld % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && ldo % 4 == 0;
     fp8_values_kernel<T><<<(unsigned)(want < most ? want : most), 256, 0, s>>>(
-        a.codes, a.rows, a.cols, a.ld, a.block_rows, a.scales, a.s_row, a.s_col, out, ldo, quads);
+        a.codes, a.rows, a.cols, a.ld, a.block_rows, a.scales, a.s_row, a.s_col, out, ldo, quads, vec);
     return cudaGetLastError();
 }
 
