@@ -281,8 +281,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int pl = 0; pl < P; ++pl)
 #pragma unroll
                             for (int k = 0; k < kStep / 16; ++k)   // 16 rows of 128 bytes
-                                mma_bf16<2>(tmem + (uint32_t)(buf * TK), d0 + (uint64_t)(pl * (kPlaneBytes >> 4)) + 128u * k,
-                                            dx + 128u * k, idesc, in > 0 || pl > 0 || k > 0);
+                                mma_bf16(tmem + (uint32_t)(buf * TK), d0 + (uint64_t)(pl * (kPlaneBytes >> 4)) + 128u * k,
+                                         dx + 128u * k, idesc, in > 0 || pl > 0 || k > 0);
                         mma_done<2>(done(s));
                         if (last) mma_done<2>(sums_full(buf));
                     }

@@ -50,20 +50,13 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
             : "memory");
 }
 
-template <int CTAS>
+// (in a CTA pair: the weight gradient)
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    if constexpr (CTAS == 2)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
-            : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
 }
 
 // True in one lane of a converged warp. The MMA issuers run their loops with the
@@ -125,57 +118,6 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// 32 columns of this warp's 32 lanes; the values are there after tmem_wait().
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-// Waits for this warp's tensor-memory loads; the registers pass through an empty
-// statement after the wait, so that no use of them moves above it.
-template <int N>
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < N; i += 8)
-        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                          "+r"(r[i + 6]), "+r"(r[i + 7]));
-}
-
-// 80 columns of this warp's 32 lanes as 40 pairs of fp32, complete on return.
-__device__ __forceinline__ void tmem_pairs(uint32_t taddr, uint64_t (&v)[40]) {
-    asm volatile(
-        "{\n\t.reg .b32 t<80>;\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15, t16, t17, t18, t19, t20, t21, t22, t23, t24, t25, t26, t27, t28, t29, t30, t31}, [%40];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {t32, t33, t34, t35, t36, t37, t38, t39, t40, t41, t42, t43, t44, t45, t46, t47, t48, t49, t50, t51, t52, t53, t54, t55, t56, t57, t58, t59, t60, t61, t62, t63}, [%41];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t64, t65, t66, t67, t68, t69, t70, t71, t72, t73, t74, t75, t76, t77, t78, t79}, [%42];\n\t"
-        "tcgen05.wait::ld.sync.aligned;\n\t"
-        "mov.b64 %0, {t0, t1};\n\tmov.b64 %1, {t2, t3};\n\tmov.b64 %2, {t4, t5};\n\tmov.b64 %3, {t6, t7};\n\t"
-        "mov.b64 %4, {t8, t9};\n\tmov.b64 %5, {t10, t11};\n\tmov.b64 %6, {t12, t13};\n\tmov.b64 %7, {t14, t15};\n\t"
-        "mov.b64 %8, {t16, t17};\n\tmov.b64 %9, {t18, t19};\n\tmov.b64 %10, {t20, t21};\n\tmov.b64 %11, {t22, t23};\n\t"
-        "mov.b64 %12, {t24, t25};\n\tmov.b64 %13, {t26, t27};\n\tmov.b64 %14, {t28, t29};\n\tmov.b64 %15, {t30, t31};\n\t"
-        "mov.b64 %16, {t32, t33};\n\tmov.b64 %17, {t34, t35};\n\tmov.b64 %18, {t36, t37};\n\tmov.b64 %19, {t38, t39};\n\t"
-        "mov.b64 %20, {t40, t41};\n\tmov.b64 %21, {t42, t43};\n\tmov.b64 %22, {t44, t45};\n\tmov.b64 %23, {t46, t47};\n\t"
-        "mov.b64 %24, {t48, t49};\n\tmov.b64 %25, {t50, t51};\n\tmov.b64 %26, {t52, t53};\n\tmov.b64 %27, {t54, t55};\n\t"
-        "mov.b64 %28, {t56, t57};\n\tmov.b64 %29, {t58, t59};\n\tmov.b64 %30, {t60, t61};\n\tmov.b64 %31, {t62, t63};\n\t"
-        "mov.b64 %32, {t64, t65};\n\tmov.b64 %33, {t66, t67};\n\tmov.b64 %34, {t68, t69};\n\tmov.b64 %35, {t70, t71};\n\t"
-        "mov.b64 %36, {t72, t73};\n\tmov.b64 %37, {t74, t75};\n\tmov.b64 %38, {t76, t77};\n\tmov.b64 %39, {t78, t79};\n\t"
-        "}"
-        : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]),
-          "=l"(v[7]), "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]), "=l"(v[12]), "=l"(v[13]),
-          "=l"(v[14]), "=l"(v[15]), "=l"(v[16]), "=l"(v[17]), "=l"(v[18]), "=l"(v[19]), "=l"(v[20]),
-          "=l"(v[21]), "=l"(v[22]), "=l"(v[23]), "=l"(v[24]), "=l"(v[25]), "=l"(v[26]), "=l"(v[27]),
-          "=l"(v[28]), "=l"(v[29]), "=l"(v[30]), "=l"(v[31]), "=l"(v[32]), "=l"(v[33]), "=l"(v[34]),
-          "=l"(v[35]), "=l"(v[36]), "=l"(v[37]), "=l"(v[38]), "=l"(v[39])
-        : "r"(taddr), "r"(taddr + 32u), "r"(taddr + 64u)
-        : "memory");
-}
 // 64 columns of this warp's 32 lanes as 32 pairs of fp32, complete on return.
 __device__ __forceinline__ void tmem_pairs(uint32_t taddr, uint64_t (&v)[32]) {
     asm volatile(
