@@ -19,7 +19,7 @@ PRODUCTS = {
     **{(m, 1003, 14333): ("few rows", 64, 1) for m in (33, 48, 49, 63, 64)},
     (3, 40000, 2000): ("few rows", 16, 1),      # a CTA's run holds whole tiles
     (20, 40000, 2000): ("few rows", 32, 1),
-    (50, 20000, 2000): ("few rows", 64, 1),
+    (50, 28672, 4096): ("few rows", 64, 1),
     (32, 20000, 8000): ("few rows", 32, 1),     # long runs: each ring wraps around many times
     (300, 130, 20001): ("pairs", 128, 8),
     (100, 777, 20000): ("pairs", 128, 8),

@@ -22,6 +22,17 @@ def test_sizes_take_the_kernels_they_test(wq) -> None:
             assert wq._kernels.fp8_weight_grad_plan(*size, dtype) == plan, size
 
 
+def test_the_faster_kernel_at_64_rows(wq) -> None:
+    """Weights for which one of the two kernels was measured at least a tenth faster than the other."""
+    for n, k in ((28672, 8192), (8192, 28672), (60000, 4000), (128256, 4096), (16384, 16384), (1024, 14336),
+                 (20000, 8000), (4096, 11008)):
+        for m in (33, 48, 64):
+            assert wq._kernels.fp8_gemm_plan(m, n, k)[0] == "few rows", (m, n, k)
+    for n, k in ((4096, 4096), (14336, 4096), (5120, 5120), (8192, 8192), (24000, 1000), (2304, 768), (50257, 768)):
+        for m in (33, 48, 64):
+            assert wq._kernels.fp8_gemm_plan(m, n, k)[0] == "pairs", (m, n, k)
+
+
 def test_plan_c_refusals(wq) -> None:
     lib = wq._kernels.library()
     a, b, c = (ctypes.c_int() for _ in range(3))

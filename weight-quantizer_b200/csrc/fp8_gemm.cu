@@ -946,14 +946,19 @@ size_t few_part_bytes(int64_t M, int64_t N, int64_t K) {
 size_t few_arrived_bytes(int64_t N) { return round_up((size_t)few_tiles(N) * 4); }
 
 // Which of the two kernels: the shorter by the pairs' model above and this one, from
-// memory, not L2: 8, a unit's time for each unit of a CTA's run, and the CTAs that
-// share a tile. Measured, wide pairs / few rows: 28672 x 8192 at 16 rows 60 / 48, at 64
-// rows 66 / 58; 11008 x 4096 at 64 rows 19 / 25; 2304 x 768 6 / 8.
+// memory, not L2: a call's fixed part, a unit's time for each unit of a CTA's run, and the
+// CTAs that share a tile; two CTAs of an SM at up to 32 rows take a unit each in the time.
+// Measured in a replayed graph over weights from memory, pairs / few rows: 28672 x 8192 at
+// 16 rows 63 / 49, at 64 rows 64 / 53; at 64 rows 60000 x 4000 67 / 55, 1024 x 14336
+// 32 / 20, 40000 x 2000 32 / 34, 11008 x 4096 21 / 22, 4096 x 4096 12 / 19. (Of 26 weights
+// at 33 to 64 rows the rule takes the slower kernel for one, by 4%.)
 double few_us(int64_t M, int64_t N, int64_t K) {
     const int64_t blocks = (K + 127) / 128, units = few_tiles(N) * blocks;
     const double run = (double)units / (double)few_ctas(N, K, few_resident(M));
     const double shared = (double)blocks / run;   // CTAs on a tile
-    return 8.0 + run * (M <= 32 ? 0.86 : 0.54) + (shared > 1.0 ? shared * (M <= 16 ? 0.5 : (M <= 32 ? 0.7 : 1.2)) : 0.0);
+    const double per_cta = shared > 1.0 ? shared : 0.0;
+    if (M > 32) return 13.5 + run * 0.39 + per_cta * 0.6;
+    return 8.0 + run * 0.86 + per_cta * (M <= 16 ? 0.5 : 0.7);
 }
 bool few_rows(int64_t M, int64_t N, int64_t K) { return M <= kFewMaxRows && few_us(M, N, K) <= pair_plan(M, N, K).us; }
 
