@@ -6,6 +6,7 @@ import copy
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch import nn
 
 from test_fp8_gpu import DTYPES, E4M3, check_product, rand, values64
@@ -210,3 +211,50 @@ def test_dequantize_rounds_once(wq, cuda) -> None:
         down = torch.nextafter(got.to(dtype), torch.full_like(got, -float("inf")).to(dtype)).double()
         err = (got - want).abs()
         assert bool((err <= (up - want).abs()).all()) and bool((err <= (down - want).abs()).all()), dtype
+
+
+# ---- sides of no length, scales of no stride, recomputation ---------------------------------------
+
+
+def test_layer_without_rows_or_sides(wq, cuda) -> None:
+    """No rows: gradients of zeros. No outputs, no inputs: what is left of the sums."""
+    w, b = rand((64, 96), 1).requires_grad_(), rand((64,), 2).requires_grad_()
+    for lead in ((0,), (3, 0)):
+        x = torch.empty(*lead, 96, device=cuda, requires_grad=True)
+        y = wq.fp8_linear(x, w, b)
+        assert y.shape == (*lead, 64)
+        dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+        assert dx.shape == x.shape and bool((dw == 0).all()) and bool((db == 0).all())
+    x, none = rand((5, 96), 3).requires_grad_(), torch.empty(0, 96, device=cuda, requires_grad=True)
+    y = wq.fp8_linear(x, none)
+    dx, dw = torch.autograd.grad(y.sum(), (x, none))
+    assert y.shape == (5, 0) and bool((dx == 0).all()) and dw.shape == (0, 96)
+    x, none = torch.empty(5, 0, device=cuda, requires_grad=True), torch.empty(64, 0, device=cuda, requires_grad=True)
+    y = wq.fp8_linear(x, none, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, none, b))
+    assert torch.equal(y, b.expand(5, 64)) and dx.shape == (5, 0) and dw.shape == (64, 0) and bool((db == 5).all())
+
+
+def test_one_scale_for_all_blocks(wq, cuda) -> None:
+    """Scales without strides: one value stands for every block."""
+    one = torch.full((1, 1), 0.375, device=cuda)
+    q, w8 = wq.quantize_fp8(rand((40, 700), 1)), wq.quantize_fp8(rand((260, 700), 2), block_rows=128)
+    a, w = wq.Fp8Blocks(q.codes, one.expand(40, 6)), wq.Fp8Blocks(w8.codes, one.expand(3, 6), 128)
+    assert torch.equal(wq.dequantize_fp8(a).double(), q.codes.double() * 0.375)
+    check_product(wq.fp8_gemm(a, w, out_dtype=torch.float32), values64(a), values64(w).t())
+    dy = rand((40, 33), 3)
+    # 0.375 has two bits: code * scale is exact in bf16
+    check_product(wq.fp8_weight_grad(dy, a), dy.double().t(), values64(a))
+
+
+def test_recomputed_forward(wq, cuda) -> None:
+    """Activation checkpointing runs the forward again: the same gradients, bit for bit."""
+    w, x = rand((64, 96), 1).requires_grad_(), rand((7, 96), 2).requires_grad_()
+
+    def part(v: torch.Tensor) -> torch.Tensor:
+        return torch.relu(wq.fp8_linear(v, w))
+
+    want = torch.autograd.grad(part(x).square().sum(), (x, w))
+    y = torch.utils.checkpoint.checkpoint(part, x, use_reentrant=False)
+    got = torch.autograd.grad(y.square().sum(), (x, w))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
