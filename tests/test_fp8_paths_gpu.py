@@ -212,6 +212,21 @@ def test_weight_grad_operand_of_the_other_cta(wq, cuda, dtype) -> None:
         assert torch.equal(out, dw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(64, 2304, 768), (40, 4096, 4096)])
+def test_weight_grad_terms_add_up_from_the_least(wq, cuda, M: int, N: int, K: int, dtype) -> None:
+    """One step of rows, all products positive. dy's terms are 2^-8 and 2^-16 of it, and the sums of the lesser ones are
+    in place before the first term's four additions (16 rows each), so those four are the only ones of the result's
+    size: each off by at most a step, 2^-23 of it, the others by 2^-8 of that, then the fp32 registers' rounding by
+    half a step. Were the first term added first, all twelve additions would cut at the result's size."""
+    dy = rand((M, N), 1, dtype).abs()
+    x = wq.quantize_fp8(rand((M, K), 2, torch.bfloat16).abs())
+    dw = wq.fp8_weight_grad(dy, x)
+    ref = dy.double().t() @ values64(x)
+    steps = 4 * (1 + 2.0 ** -7 + 2.0 ** -15) + 0.5
+    assert bool(((dw.double() - ref).abs() <= steps * 2.0 ** -23 * ref).all())
+
+
 @pytest.mark.parametrize("M,N,K", [(200, 4096, 4096), (777, 300, 520), (5000, 256, 384)])
 def test_weight_grad_any_scales(wq, cuda, M: int, N: int, K: int) -> None:
     """Scales that are no powers of two: each code * scale is rounded to bfloat16 (by half a step, 2^-8, after a
