@@ -352,8 +352,9 @@ WQ_API int wq_dequant_gemm_f32_multi(const float* x, int64_t B, int64_t K,
 /*           is scales[(r / block_rows) * s_row + (c / 128) * s_col]; any    */
 /*           non-negative strides. The last block of a row or column may be  */
 /*           short.                                                          */
-/* and stands for code * scale. The products take any finite fp32 scales     */
-/* whose product is finite too. Codes of a product's operand start on a      */
+/* and stands for code * scale. The products take any fp32 scales, as long   */
+/* as the product of two blocks' scales is a normal number: they are         */
+/* multiplied first, and an infinite product times a sum of 0 is NaN. Codes of a product's operand start on a      */
 /* 16-byte boundary and ld is a multiple of 16 (pad the rows; what the       */
 /* padding holds is not read as a value). Sums are held in fp32; every       */
 /* result is rounded once to its type and the same on every call.            */

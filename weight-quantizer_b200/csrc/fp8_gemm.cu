@@ -3,8 +3,9 @@
 //   y[m, n] = sum_b sa[m, b] sb[n / 128, b] sum_{k in block b} a[m, k] w[n, k] (+ bias[n])
 //
 // A block's sum over 128 products runs on the tensor cores (e4m3 x e4m3, fp32 in
-// tensor memory); the scales cannot enter there, so each block's sum is read back
-// and added to fp32 registers, times the product of its two scales.
+// tensor memory); scales of any fp32 value cannot enter there (the block-scaled MMA
+// takes powers of two alone), so each block's sum is read back and added to fp32
+// registers, times the product of its two scales.
 #include "fp8_types.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"

@@ -11,8 +11,10 @@
 // and the product code * scale become exact: the weight gradient reads
 // code * scale as a bf16 operand without a rounding.
 //
-// Bound: HBM. Bytes per value: the input's 2 or 4, 1 for the code, 4/128 (rows)
-// or 4/16384 (tiles) for the scale.
+// Bytes per value: the input's 2 or 4, 1 for the code, 4/128 (rows) or 4/16384 (tiles) for
+// the scale. Tiles are bound by them (28672 x 8192 fp32 205 us, 179 at the copy rate), rows by
+// instructions, the shuffles, vote and scale of each eight values (4096 x 8192 bf16 24 us,
+// 15.5 at the copy rate).
 #include "fp8_types.cuh"
 #include "kernels.h"
 #include "launch.h"

@@ -9,8 +9,9 @@ values of a row (``block_rows=1``), weights one per 128 x 128 tile
     y[m, n] = sum_b sa[m, b] * sw[n // 128, b] * sum_{k in block b} a[m, k] * w[n, k]
 
 ``quantize_fp8`` makes such operands (its scales are powers of two, so dividing
-by one loses nothing); the products take operands with any scales, such as a
-checkpoint's. ``fp8_linear`` is the differentiable layer: its forward product
+by one loses nothing); the products take operands with other scales too, such as
+a checkpoint's, as long as ``sa * sw`` is a normal fp32 number (it is computed
+first). ``fp8_linear`` is the differentiable layer: its forward product
 reads the input in 8 bits, and the same codes, one byte per value instead of
 two or four, are all that it keeps of the input for the weight's gradient:
 
@@ -84,6 +85,7 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1) -> Fp8Blocks:
     A block's scale is the least power of two s >= 2^-117 with max|x| <= 448 s
     over its finite values (1 for a block of zeros); a code is the e4m3 value
     nearest to x / s, ties to even. NaN and infinities become the NaN code.
+    (From 2^128 (1 - 2^-5) on a value's code stands for 2^128, beyond float32.)
     """
     if block_rows not in _BLOCK_ROWS:
         raise ValueError("block_rows must be 1 or 128")
@@ -147,7 +149,8 @@ def fp8_weight_grad(
     [rows, in] (``block_rows=1``).
 
     With ``quantize_fp8``'s scales no operand is rounded (x's values are exact in
-    bfloat16, and a 32-bit ``dy`` enters the product as a sum of bfloat16 terms);
+    bfloat16, and a 16- or 32-bit ``dy`` enters the product as a sum of bfloat16
+    terms, down to bits of 2^-133);
     other scales' ``code * scale`` is rounded to bfloat16. ``accumulate`` adds to
     ``out``, in ``out``'s type.
     """
