@@ -410,17 +410,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     const float2 f = unpack2(acc[2 * k]), g = unpack2(acc[2 * k + 1]);
                     mine[k * 128] = make_float4(f.x, f.y, g.x, g.y);
                 }
-                __threadfence();
                 named_barrier(1, 256);
                 volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
                 const int tile = t / splits;
                 if (warp == 4 && lane == 0)
-                    *flag = atomicAdd(p.arrived + tile * 2 + rank, 1u) == (unsigned)(splits - 1);
+                    *flag = last_to_arrive(p.arrived + tile * 2 + rank, (unsigned)splits);
                 named_barrier(1, 256);
                 write = *flag != 0u;
                 named_barrier(1, 256);   // the flag has been read
                 if (write) {
-                    __threadfence();
 #pragma unroll
                     for (int k = 0; k < C / 2; ++k) acc[k] = 0;
                     const uint64_t one = pack2(1.0f, 1.0f);
@@ -735,16 +733,14 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::CTAS)
                     p.part + (2 * (int64_t)blockIdx.x + (from == u0 ? 0 : 1)) * (128 * BN) + lane_at);
 #pragma unroll
                 for (int c = 0; c < C / 4; ++c) mine[c * 128] = y[c];
-                __threadfence();
                 named_barrier(1, 32 * L::SUM_WARPS);
                 volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
                 const int64_t c0 = cta_of(t0, p.units, ctas), c1 = cta_of(t1 - 1, p.units, ctas);
-                if (warp == 4 && lane == 0) *flag = atomicAdd(p.arrived + tile, 1u) == (unsigned)(c1 - c0);
+                if (warp == 4 && lane == 0) *flag = last_to_arrive(p.arrived + tile, (unsigned)(c1 - c0 + 1));
                 named_barrier(1, 32 * L::SUM_WARPS);
                 write = *flag != 0u;
                 named_barrier(1, 32 * L::SUM_WARPS);   // the flag has been read
                 if (write) {
-                    __threadfence();
 #pragma unroll
                     for (int c = 0; c < C / 4; ++c) y[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     // (several CTAs' sums are on their way at once)

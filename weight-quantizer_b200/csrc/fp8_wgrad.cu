@@ -451,17 +451,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < TK / 8; ++c)
                     mine[c * 128] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
-                __threadfence();
                 named_barrier(1, 256);
                 volatile uint32_t* flag = reinterpret_cast<volatile uint32_t*>(smem + L::FLAG);
                 const int tile = t / splits;
                 if (warp == 12 && lane == 0)
-                    *flag = atomicAdd(p.arrived + tile * 2 + rank, 1u) == (unsigned)(splits - 1);
+                    *flag = last_to_arrive(p.arrived + tile * 2 + rank, (unsigned)splits);
                 named_barrier(1, 256);
                 write = *flag != 0u;
                 named_barrier(1, 256);   // the flag has been read
                 if (write) {
-                    __threadfence();
 #pragma unroll
                     for (int c = 0; c < TK / 2; ++c) acc[c] = 0.0f;
 #pragma unroll 1

@@ -230,6 +230,17 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// Arrival of a CTA whose warps have stored partial sums to global memory and met at a
+// barrier of theirs: true for the last of `all`. The first fence covers what the barrier
+// ordered before it, every warp's sums; the second the other CTAs' sums, for the warps
+// that this thread meets at the next barrier. By one thread.
+__device__ __forceinline__ bool last_to_arrive(unsigned int* arrived, unsigned int all) {
+    __threadfence();
+    const bool last = atomicAdd(arrived, 1u) == all - 1u;
+    __threadfence();
+    return last;
+}
+
 // ---- CTA pairs -----------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
