@@ -10,8 +10,8 @@ values of a row (``block_rows=1``), weights one per 128 x 128 tile
 
 ``quantize_fp8`` makes such operands (its scales are powers of two, so dividing
 by one loses nothing); the products take operands with other scales too, such as
-a checkpoint's, as long as ``sa * sw`` is a normal fp32 number (it is computed
-first). ``fp8_linear`` is the differentiable layer: its forward product
+a checkpoint's, as long as ``sa * sw`` is a normal fp32 number or 0 (it is
+computed first). ``fp8_linear`` is the differentiable layer: its forward product
 reads the input in 8 bits, and the same codes, one byte per value instead of
 two or four, are all that it keeps of the input for the weight's gradient:
 
