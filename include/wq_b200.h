@@ -356,8 +356,8 @@ WQ_API int wq_dequant_gemm_f32_multi(const float* x, int64_t B, int64_t K,
 /* as the product of two blocks' scales is a normal number or 0: they are    */
 /* multiplied first, and an infinite product times a sum of 0 is NaN. Codes  */
 /* of a product's operand start on a 16-byte boundary and ld is a multiple   */
-/* of 16 (pad the rows; the padding is not read as values). Sums are held in fp32; every       */
-/* result is rounded once to its type and the same on every call.            */
+/* of 16 (pad the rows; the padding is not read as values). Sums are held in */
+/* fp32; every result is rounded once to its type and the same on every call. */
 /* Workspaces are 256-byte aligned device memory of the queried size (none   */
 /* where that is 0), WQ_E_WORKSPACE otherwise, and serve one call at a time. */
 /* ------------------------------------------------------------------------ */
